@@ -178,7 +178,11 @@ __global__ __launch_bounds__(256) void time_warp_kernel(const float* __restrict_
     fy -= (float)sy;
     const int s0 = min(max(sy, 0), src - 1), s1 = min(max(sy + 1, 0), src - 1);
     const float a = xb[(int64_t)(seg0 + s0) * C + c], bb = xb[(int64_t)(seg0 + s1) * C + c];
-    yb[idx] = __fadd_rn(__fmul_rn(a, 1.0f - fy), __fmul_rn(bb, fy));  // no contraction: the oracle's two products and a sum
+    {
+#pragma clang fp contract(off)  // the oracle's two products and a sum (__fmul_rn / __fadd_rn alone do not keep hipcc from an fma)
+      const float lo = a * (1.0f - fy), hi = bb * fy;
+      yb[idx] = lo + hi;
+    }
   }
 }
 
