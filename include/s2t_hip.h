@@ -780,6 +780,83 @@ typedef struct s2t_rowblock_dgrad_args {
 } s2t_rowblock_dgrad_args;
 int s2t_rowblock_dgrad(const s2t_rowblock_dgrad_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Paged key/value cache of an incremental decoder, and attention of several new tokens of a sequence over it.
+ *
+ * Replaces, for a decoder that pushes more than one token per pass (verification of drafted tokens) or shares its memory among many
+ * sequences, the concatenated and re-ordered caches of modules/multihead_attention.py:302-339,574-592 and the bmm / softmax / bmm
+ * behind them (:367-420); the rotation is modules/rotary_positional_embedding.py's (halves, not interleaved).
+ *
+ * A page holds page_size (a power of two) consecutive places of one sequence for every key/value head:
+ * element (page, head, place, c) at page * p_sp + head * p_sh + place * p_sr + c of k_pages / v_pages.  page_table[b * table_stride + i]
+ * names the page of places i * page_size ..; lens[b] is the length of sequence b INCLUDING its new tokens; the rows cu[b] ..
+ * cu[b + 1] - 1 of the new tokens' arrays are those of sequence b, in order: row cu[b] + i sits at place lens[b] - (cu[b + 1] - cu[b]) + i.
+ * table, lens, cu, positions, rows and tree are read on the device, so one captured graph serves batches of any fill below B, N and
+ * max_new; rows from cu[B] on are left as they were.  What they say is bounded on the device: a new token whose place is negative,
+ * beyond the table, or on a page outside 0 .. num_pages - 1 is not stored; a key there does not exist; rows beyond N or beyond max_new of
+ * their sequence are not computed.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct s2t_paged_args {
+  int32_t dtype;          /* S2T_F32 / S2T_BF16: of the pages and of q, k, v, q_out, out */
+  int32_t B;              /* sequences */
+  int32_t N;              /* rows of the new tokens' arrays */
+  int32_t max_new;        /* no sequence has more new tokens than this (launch bound) */
+  int32_t q_heads, kv_heads, dk; /* q_heads % kv_heads == 0: query head h reads key/value head h / (q_heads / kv_heads); dk % 16 == 0, <= 256 */
+  int32_t num_pages, page_size, table_pages; /* table_pages: entries of a page_table row */
+  void* k_pages;
+  void* v_pages;
+  int64_t p_sp, p_sh, p_sr;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* lens;    /* [B] */
+  const int32_t* cu;      /* [B + 1] */
+  /* s2t_paged_kv_append: k, v (and q, or NULL) [rows][heads][dk] with row and head strides */
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const void* q;          /* attention: the queries; append: optional, rotated into q_out */
+  int64_t q_st, q_sh;
+  void* q_out;
+  int64_t qo_st, qo_sh;
+  const float* rotary;    /* [rotary_positions][rot_dim]: rot_dim / 2 cosines, then the sines; NULL: no rotation */
+  int32_t rotary_positions, rot_dim; /* rot_dim % 16 == 0, <= dk: elements i and i + rot_dim / 2 turn together, the rest passes */
+  const int32_t* positions; /* optional [N]: position of each new token's rotation (default: its place); outside the table: NaN is stored */
+  const int32_t* rows;    /* optional [N]: new token t takes row rows[t] of k and v (< 0 or >= src_rows: not stored); not with q */
+  int32_t src_rows;
+  /* s2t_paged_attention */
+  void* out;              /* [N][q_heads][dk] */
+  int64_t o_st, o_sh;
+  float* lse;             /* optional [N][q_heads]: log of the sum of exp(score) (-inf for a row that sees nothing; its output is 0) */
+  const int64_t* tree;    /* optional [N][tree_stride]: bit j of row t's words = it sees new token j of its sequence; NULL: all up to itself */
+  int64_t tree_stride;
+  int32_t tree_words;     /* words of a row that exist; new tokens beyond 64 * tree_words are not seen */
+  float scale;
+  void* ws;               /* s2t_paged_attention_ws_bytes(args) bytes, 16-byte aligned; contents undefined before and after */
+  int64_t ws_bytes;
+} s2t_paged_args;
+/* k | v of the new tokens into their pages, rotated on the way; q rotated into q_out (q_out == q with equal strides: in place) */
+int s2t_paged_kv_append(const s2t_paged_args* args, void* stream);
+/* out = softmax(scale * q k^T) v over the keys a row sees, fp32 scores and statistics */
+int s2t_paged_attention(const s2t_paged_args* args, void* stream);
+int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* args);
+
+/* ------------------------------------------------------------------------------------------------
+ * Scores of given tokens (sequence_scorer.py:75-110; the log_softmax + topk of search.py:113-146 per row): with z = inv_temp * logits,
+ *   lse[r] = log sum exp z[r],  logprob[r] = z[r][tokens[r]] - lse[r],  entropy[r] = - sum p log p,
+ *   top_index[r][0 .. top) = the columns of the largest logits, equal ones by ascending column, top_logprob their z - lse.
+ * All in fp32 from one pass over the row (top <= 64).  tokens may be NULL (no logprob).  A row whose token is ignore_index scores 0,
+ * top_index -1, and is not read; a token outside 0 .. V - 1 gives NaN.  Any of logprob, lse, entropy may be NULL.
+ * _bwd: dlogits for upstream gradients g_logprob, g_entropy ([rows], or NULL) and g_top ([rows][top], or NULL) from the saved lse and
+ * entropy (needed with g_entropy only); every element of dlogits[rows][V] is written, zeros in ignored rows.
+ * ------------------------------------------------------------------------------------------------ */
+int s2t_token_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore_index,
+                           float inv_temp, int top, float* logprob, float* lse, float* entropy, float* top_logprob, int64_t* top_index,
+                           void* stream);
+int s2t_token_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore_index,
+                           float inv_temp, int top, const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy,
+                           const float* g_top, const int64_t* top_index, void* dlogits, int64_t ldd, void* stream);
+
 /* ---- Gradient all-reduce over RCCL / xGMI (csrc/comm.hip) ------------------------------------------------
  * Replaces torch.distributed.all_reduce in LegacyDistributedDataParallel.all_reduce_grads
  * (distributed/legacy_distributed_data_parallel.py:107-120): one process-global communicator (one process per GPU),

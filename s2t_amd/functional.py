@@ -9,10 +9,12 @@ There is no CPU path: every function raises if its inputs are not on the GPU.
 """
 import math
 import os
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import kernels as K
+from ._lib import require_cuda
 from .flat_params import cw, transposed
 
 _HOOKS = {"grad_ready": None}  # set by the DDP wrapper: called with a parameter once its gradient is final
@@ -2312,6 +2314,84 @@ def label_smoothed_ce(logits, target, eps, pad_idx, rows=None):
 
 
 _SIDE = {"streams": {}, "pending": []}
+
+
+class TokenScores(NamedTuple):
+    """What ``token_logprobs`` returns; fields that were not asked for are None."""
+
+    logprob: Optional[torch.Tensor]      # [...] fp32
+    entropy: Optional[torch.Tensor]      # [...] fp32
+    top_logprob: Optional[torch.Tensor]  # [..., top] fp32
+    top_index: Optional[torch.Tensor]    # [..., top] int64
+
+
+NO_IGNORE = -(1 << 63)
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    """Log probabilities of ``tokens`` under rows of logits, entropies and the best alternatives, and their gradient
+    (sequence_scorer.py:75-110); the row statistics are saved, the probabilities are formed again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, ignore_index, inv_temp, top, want_entropy):
+        rows, V = logits.shape
+        f32 = dict(dtype=torch.float32, device=logits.device)
+        logprob = torch.empty(rows, **f32) if tokens is not None else None
+        train = ctx.needs_input_grad[0]
+        lse = torch.empty(rows, **f32) if train else None
+        entropy = torch.empty(rows, **f32) if want_entropy else None
+        top_lp = torch.empty(rows, top, **f32) if top else None
+        top_idx = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
+        K.token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_lp, top_idx)
+        if train:
+            ctx.save_for_backward(logits, tokens, lse, entropy, top_idx)
+            ctx.args = (ignore_index, inv_temp, top)
+            ctx.set_materialize_grads(False)
+            if top_idx is not None:
+                ctx.mark_non_differentiable(top_idx)
+        return logprob, entropy, top_lp, top_idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprob, g_entropy, g_top, _):
+        logits, tokens, lse, entropy, top_idx = ctx.saved_tensors
+        ignore_index, inv_temp, top = ctx.args
+        if g_logprob is None and g_entropy is None and g_top is None:
+            return (None,) * 6
+        dl = torch.empty(logits.shape[0], _pad8(logits.shape[1]), dtype=logits.dtype, device=logits.device)[:, :logits.shape[1]]
+        g_logprob, g_entropy, g_top = (g.contiguous() if g is not None else None for g in (g_logprob, g_entropy, g_top))
+        K.token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_idx, dl)
+        return dl, None, None, None, None, None
+
+
+def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, ignore_index=None):
+    """Scores of given tokens: ``log_softmax(logits / temperature)`` at ``tokens``, with the entropy of every row and its ``top``
+    (at most 64) best columns, equal logits in ascending order.  ``logits`` [..., V] fp32 or bf16 with any row stride (a view of
+    rows padded to a multiple of 8, as the output projection returns them, is read in place), ``tokens`` [...] int64.
+    Rows whose token is ``ignore_index`` score 0 (top_index -1), are not read and get no gradient; a token outside the vocabulary scores
+    NaN.  All results are fp32, differentiable with respect to the logits (once).  -> ``TokenScores``"""
+    if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("token_logprobs: logits [..., V] in float32 or bfloat16 expected, got %s %s" % (tuple(logits.shape), logits.dtype))
+    V, lead = logits.shape[-1], logits.shape[:-1]
+    if V < 1 or not 0 <= top <= min(V, 64):
+        raise ValueError("token_logprobs: top = %s of a vocabulary of %d (at most 64)" % (top, V))
+    if not temperature > 0 or temperature == math.inf:
+        raise ValueError("token_logprobs: temperature must be positive, got %s" % temperature)
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != lead or tokens.device != logits.device):
+        raise ValueError("token_logprobs: tokens must be int64 of shape %s on %s, got %s %s on %s" % (
+            tuple(lead), logits.device, tokens.dtype, tuple(tokens.shape), tokens.device))
+    if tokens is None and not top and not entropy:
+        raise ValueError("token_logprobs: nothing asked for (tokens, top or entropy)")
+    require_cuda(logits, tokens)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.shape[0] and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
+        x = x.contiguous()
+    y = None if tokens is None else tokens.reshape(-1).contiguous()
+    r = TokenLogprobsFn.apply(x, y, NO_IGNORE if ignore_index is None else int(ignore_index), 1.0 / temperature, int(top), bool(entropy))
+    if logits.dim() == 2:
+        return TokenScores(*r)
+    shape = lambda t: None if t is None else t.view(lead + t.shape[1:])  # noqa: E731
+    return TokenScores(*(shape(t) for t in r))
 
 
 def _side_stream(device):

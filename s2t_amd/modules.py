@@ -568,6 +568,13 @@ def rel_pos_table(T: int, dim: int) -> torch.Tensor:
     return tab
 
 
+def rotary_table(n_pos: int, dim: int, base: float = 10000.0) -> torch.Tensor:
+    """modules/rotary_positional_embedding.py — row p: cos(p w_i), then sin(p w_i), w_i = base^(-2i/dim); angles in 64 bits (in 32 the
+    angle of position 10^5 is off by 0.004)."""
+    ang = torch.arange(n_pos, dtype=torch.float64)[:, None] * base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    return torch.cat([torch.cos(ang), torch.sin(ang)], dim=1).float()
+
+
 class _TableCache:
     def __init__(self):
         self.c = {}
@@ -575,7 +582,7 @@ class _TableCache:
     def get(self, kind, n, dim, device, dtype=torch.float32):
         key = (kind, n, dim, str(device), dtype)
         if key not in self.c:
-            t = sinusoidal_table(n, dim) if kind == "sin" else rel_pos_table(n, dim)
+            t = {"sin": sinusoidal_table, "rotary": rotary_table}.get(kind, rel_pos_table)(n, dim)
             self.c[key] = t.to(device=device, dtype=dtype)
         return self.c[key]
 

@@ -1,0 +1,156 @@
+"""Paged key/value cache of an incremental decoder and attention of several new tokens of a sequence over it.
+
+The reference's decoder keeps one dense key/value buffer per layer, takes one token per pass and copies the buffers when hypotheses change
+places (modules/multihead_attention.py:302-339,574-592).  Here the memory of a layer is a pool of pages that a table deals out to
+sequences, and a pass may bring any number of new tokens to each of them: a prompt, the next token, or DRAFTED tokens — a chain
+(a CTC transcript) or a tree of alternatives — of which the accepted ones are taken over afterwards.
+
+All functions work on the tensors a serving program keeps:
+
+* ``k_pages`` / ``v_pages`` ``[pages, kv_heads, page_size, head_dim]`` float32 or bfloat16, last dimension contiguous, equal strides (a
+  permuted view of ``[pages, page_size, kv_heads, head_dim]`` will do); page_size a power of two, head_dim a multiple of 16 up to 256;
+* ``page_table`` ``[seqs, n]`` int32: page of the places ``i * page_size ..`` of each sequence; unused entries may hold anything;
+* ``lens`` ``[seqs]`` int32: length of each sequence INCLUDING its new tokens;
+* ``cu`` ``[seqs + 1]`` int32: the new tokens' rows of sequence b are ``cu[b] .. cu[b + 1] - 1``, the last one at place ``lens[b] - 1``;
+* ``max_new``: no sequence brings more new tokens than this (a launch bound: later ones of a sequence are left out).
+
+What table, lens, cu, tree, positions and rows say is read on the device, so a captured graph serves batches of any fill; rows behind the
+last sequence are left as they were, and an entry that leads out of its bounds is never followed (include/s2t_hip.h).
+"""
+import torch
+
+from . import _lib as L
+from . import kernels as K
+
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _refuse(what):
+    raise ValueError("paged cache: " + what)
+
+
+def _check_cache(k_pages, v_pages, page_table, lens, cu, max_new):
+    if k_pages.dim() != 4 or k_pages.dtype not in _TYPES or v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape:
+        _refuse("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of one type (float32 or bfloat16), got %s %s and %s %s" % (
+            tuple(k_pages.shape), k_pages.dtype, tuple(v_pages.shape), v_pages.dtype))
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        _refuse("k_pages and v_pages need equal strides and a contiguous last dimension")
+    P, H, S, d = k_pages.shape
+    if P < 1 or H < 1 or S < 1 or S & (S - 1) or d % 16 or not 16 <= d <= 256:
+        _refuse("page_size must be a power of two and head_dim a multiple of 16 up to 256, got %s" % (tuple(k_pages.shape),))
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[1] < 1 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        _refuse("page_table must be int32 [seqs, pages of a sequence] with contiguous rows")
+    B = page_table.shape[0]
+    if lens.dtype != torch.int32 or tuple(lens.shape) != (B,) or not lens.is_contiguous():
+        _refuse("lens must be int32 [%d], contiguous" % B)
+    if cu.dtype != torch.int32 or tuple(cu.shape) != (B + 1,) or not cu.is_contiguous():
+        _refuse("cu must be int32 [%d], contiguous" % (B + 1))
+    if not 1 <= B <= 65535 or max_new < 0:
+        _refuse("1 to 65535 sequences and max_new >= 0 expected, got %d and %s" % (B, max_new))
+
+
+def _check_rows(name, t, heads, like, n=None):
+    if t.dim() != 3 or t.dtype != like.dtype or (heads is not None and t.shape[1] != heads) or t.shape[2] != like.shape[3] or t.stride(2) != 1 \
+            or (n is not None and t.shape[0] != n):
+        _refuse("%s must be [%s, %s, %d] %s with a contiguous last dimension, got %s %s" % (
+            name, "rows" if n is None else n, "heads" if heads is None else heads, like.shape[3], like.dtype, tuple(t.shape), t.dtype))
+
+
+def _check_index(name, t, n):
+    if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        _refuse("%s must be int32 [%d], contiguous" % (name, n))
+
+
+def _one_device(*tensors):
+    L.require_cuda(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            _refuse("tensors on %s and %s" % (dev, t.device))
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the paged cache is inference only: wrap the decoder in torch.no_grad()")
+
+
+def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=None, rotary=None, positions=None, rows=None, q_out=None):
+    """Stores the new tokens' keys and values ``[N, kv_heads, head_dim]`` (views of a fused projection's rows are read in place).
+
+    ``rotary`` (float32 ``[positions, rot_dim]``: cosines, then sines; ``modules.rotary_table``) turns the first rot_dim elements of every
+    key by the token's place, or by ``positions[t]`` (int32: in a tree of drafts the depth, not the place), element i together with
+    element i + rot_dim / 2; a position outside the table is stored as NaN.  ``q`` ``[N, q_heads, head_dim]`` is turned by the same call
+    into ``q_out`` (default: a new tensor; ``q`` itself: in place) and returned.
+    ``rows`` (int32 [N], instead of q): new token t takes row ``rows[t]`` of k and v — the accepted drafts of a verified tree, whose
+    projections the caller has kept; a row outside k is not stored."""
+    _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
+    _check_rows("k", k, k_pages.shape[1], k_pages)
+    _check_rows("v", v, k_pages.shape[1], k_pages, k.shape[0])
+    N = k.shape[0] if rows is None else rows.shape[0]
+    if rows is not None:
+        if q is not None:
+            _refuse("q cannot be turned together with a selection of rows")
+        _check_index("rows", rows, N)
+    if positions is not None:
+        _check_index("positions", positions, N)
+    if max_new >= 1 << 31 or N >= 1 << 31:
+        _refuse("%d new tokens" % max(N, max_new))
+    a = K.paged_args(k_pages, v_pages, page_table, lens, cu, N, max_new, k_pages.shape[1] if q is None else q.shape[1])
+    a.k, a.k_st, a.k_sh = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
+    if rotary is not None:
+        if rotary.dtype != torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.shape[0] < 1 \
+                or rotary.shape[1] % 16 or not 16 <= rotary.shape[1] <= k_pages.shape[3]:
+            _refuse("rotary must be float32 [positions, rot_dim], contiguous, rot_dim a multiple of 16 up to head_dim, got %s %s" % (
+                tuple(rotary.shape), rotary.dtype))
+        a.rotary, (a.rotary_positions, a.rot_dim) = rotary.data_ptr(), rotary.shape
+    if q is not None:
+        _check_rows("q", q, None, k_pages, N)
+        if q.shape[1] < 1 or q.shape[1] % k_pages.shape[1]:
+            _refuse("%d query heads over %d key/value heads" % (q.shape[1], k_pages.shape[1]))
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _check_rows("q_out", q_out, q.shape[1], k_pages, N)
+        a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
+        a.q_out, a.qo_st, a.qo_sh = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    elif q_out is not None:
+        _refuse("q_out without q")
+    _one_device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out)
+    if positions is not None:
+        a.positions = positions.data_ptr()
+    if rows is not None:
+        a.rows, a.src_rows = rows.data_ptr(), k.shape[0]
+    K.paged_kv_append(a, k_pages.device)
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=None, scale=None, out=None, return_lse=False):
+    """``softmax(scale * q k^T) v`` of the new tokens ``q [N, q_heads, head_dim]`` over their sequences' pages (the new tokens' own keys and
+    values have been appended): query head h reads key/value head ``h // (q_heads // kv_heads)``.
+
+    Every new token sees the whole prefix.  Of the new tokens of its sequence it sees those up to itself, or with ``tree`` (int64
+    ``[N, words]``) new token j where bit ``j % 64`` of word ``j // 64`` of its row is set — its ancestors and itself, any other set will do.
+    A row that sees nothing comes out 0 with lse -inf; what a row does not see never touches it, infinities and NaN included.
+    Inference only.  -> out [N, q_heads, head_dim] (``out`` if given), with ``return_lse`` also the fp32 logsumexp [N, q_heads]."""
+    _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
+    _check_rows("q", q, None, k_pages)
+    N, Hq, d = q.shape
+    if Hq < 1 or Hq % k_pages.shape[1] or Hq > 65535 or max_new >= 1 << 31 or N >= 1 << 31:
+        _refuse("%d query heads over %d key/value heads, %d new tokens" % (Hq, k_pages.shape[1], N))
+    a = K.paged_args(k_pages, v_pages, page_table, lens, cu, N, max_new, Hq)
+    if tree is not None:
+        if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
+            _refuse("tree must be int64 [%d, words] with contiguous rows, got %s %s" % (N, tuple(tree.shape), tree.dtype))
+        a.tree, a.tree_stride, a.tree_words = tree.data_ptr(), tree.stride(0), tree.shape[1]
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_rows("out", out, Hq, k_pages, N)
+    _one_device(k_pages, v_pages, page_table, lens, cu, q, tree, out)
+    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
+    a.out, a.o_st, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
+    a.scale = d ** -0.5 if scale is None else float(scale)
+    lse = None
+    if return_lse:
+        lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device)
+        a.lse = lse.data_ptr()
+    K.paged_attention(a, q.device)
+    return (out, lse) if return_lse else out

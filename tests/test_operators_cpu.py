@@ -1,0 +1,163 @@
+"""What the paged cache and the token scores refuse, checked on the CPU (a call that is right in every other way then asks for the GPU)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from s2t_amd import _lib as L
+from s2t_amd import functional as Fn
+from s2t_amd import modules as M
+from s2t_amd import paged
+
+
+def _struct_fields(name):
+    import re
+    src = open(L.HEADER_PATH).read()
+    start = src.index("typedef struct %s {" % name) + len("typedef struct %s {" % name)
+    body = re.sub(r"/\*.*?\*/", "", src[start:src.index("} %s;" % name)], flags=re.S)
+    names = []
+    for decl in body.split(";"):
+        parts = decl.replace("*", " ").strip().split(",")
+        if parts[0].strip():
+            names += [parts[0].split()[-1]] + [p.strip() for p in parts[1:]]
+    return names
+
+
+def test_paged_struct_matches_header_field_order():
+    assert _struct_fields("s2t_paged_args") == [f[0] for f in L.PagedArgs._fields_]
+
+
+def _good(dtype=torch.float32, B=3, N=5, H=2, Hq=4, d=32, S=16, P=7):
+    return dict(k=torch.zeros(N, H, d, dtype=dtype), v=torch.zeros(N, H, d, dtype=dtype), k_pages=torch.zeros(P, H, S, d, dtype=dtype),
+                v_pages=torch.zeros(P, H, S, d, dtype=dtype), page_table=torch.zeros(B, 2, dtype=torch.int32),
+                lens=torch.ones(B, dtype=torch.int32), cu=torch.zeros(B + 1, dtype=torch.int32), max_new=2)
+
+
+def _attend(**change):
+    a = _good()
+    a.pop("k"), a.pop("v")
+    a["q"] = torch.zeros(5, 4, 32)
+    a.update(change)
+    return paged.paged_attention(a.pop("q"), **a)
+
+
+def _append(**change):
+    a = _good()
+    a.update(change)
+    return paged.paged_kv_append(**a)
+
+
+def test_good_calls_ask_for_the_gpu():
+    for call in (_attend, _append, lambda: _append(rotary=M.rotary_table(8, 32), q=torch.zeros(5, 4, 32)), lambda: _attend(tree=torch.zeros(5, 1, dtype=torch.int64), return_lse=True),
+                 lambda: Fn.token_logprobs(torch.zeros(2, 9), torch.zeros(2, dtype=torch.int64), top=3)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+i32 = torch.int32
+BAD_CACHE = [
+    dict(k_pages=torch.zeros(7, 2, 16, 32, dtype=torch.float16), v_pages=torch.zeros(7, 2, 16, 32, dtype=torch.float16)),
+    dict(v_pages=torch.zeros(7, 2, 16, 32, dtype=torch.bfloat16)),
+    dict(v_pages=torch.zeros(8, 2, 16, 32)),
+    dict(v_pages=torch.zeros(7, 16, 2, 32).transpose(1, 2)),                     # other strides than k_pages
+    dict(k_pages=torch.zeros(7, 2, 12, 32), v_pages=torch.zeros(7, 2, 12, 32)),  # not a power of two
+    dict(k_pages=torch.zeros(7, 2, 16, 24), v_pages=torch.zeros(7, 2, 16, 24)),
+    dict(k_pages=torch.zeros(7, 2, 16, 272), v_pages=torch.zeros(7, 2, 16, 272)),
+    dict(k_pages=torch.zeros(7, 2, 16), v_pages=torch.zeros(7, 2, 16)),
+    dict(k_pages=torch.zeros(0, 2, 16, 32), v_pages=torch.zeros(0, 2, 16, 32)),
+    dict(page_table=torch.zeros(3, 2, dtype=torch.int64)),
+    dict(page_table=torch.zeros(3, 0, dtype=i32)),
+    dict(page_table=torch.zeros(2, 3, dtype=i32).t()),
+    dict(lens=torch.ones(4, dtype=i32)),
+    dict(lens=torch.ones(3, dtype=torch.int64)),
+    dict(cu=torch.zeros(3, dtype=i32)),
+    dict(cu=torch.zeros(8, dtype=i32)[::2]),
+    dict(max_new=-1),
+    dict(max_new=1 << 31),
+    dict(page_table=torch.zeros(0, 2, dtype=i32), lens=torch.ones(0, dtype=i32), cu=torch.zeros(1, dtype=i32)),
+]
+
+
+@pytest.mark.parametrize("change", BAD_CACHE)
+def test_bad_caches_are_refused(change):
+    for call in (_append, _attend):
+        with pytest.raises(ValueError, match="paged cache"):
+            call(**change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=torch.zeros(5, 3, 32)), dict(k=torch.zeros(5, 2, 64)), dict(k=torch.zeros(5, 2, 32, dtype=torch.bfloat16)), dict(k=torch.zeros(5, 64)),
+    dict(v=torch.zeros(4, 2, 32)), dict(v=torch.zeros(5, 2, 64)[..., ::2]), dict(q=torch.zeros(5, 3, 32)), dict(q=torch.zeros(4, 4, 32)),
+    dict(q=torch.zeros(5, 4, 32), q_out=torch.zeros(5, 2, 32)), dict(q_out=torch.zeros(5, 4, 32)),
+    dict(q=torch.zeros(5, 4, 32), rows=torch.zeros(5, dtype=i32)), dict(rows=torch.zeros(5, dtype=torch.int64)), dict(rows=torch.zeros(10, dtype=i32)[::2]),
+    dict(positions=torch.zeros(4, dtype=i32)), dict(rows=torch.zeros(3, dtype=i32), positions=torch.zeros(5, dtype=i32)),
+    dict(rotary=torch.zeros(9, 24)), dict(rotary=torch.zeros(9, 48)), dict(rotary=torch.zeros(9, 32, dtype=torch.float64)), dict(rotary=torch.zeros(0, 32)),
+    dict(rotary=torch.zeros(9, 64)[:, ::2])])
+def test_bad_appends_are_refused(change):
+    with pytest.raises(ValueError, match="paged cache"):
+        _append(**change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros(5, 3, 32)), dict(q=torch.zeros(5, 0, 32)), dict(q=torch.zeros(5, 4, 16)), dict(q=torch.zeros(5, 4, 32, dtype=torch.bfloat16)),
+    dict(q=torch.zeros(5, 4, 64)[..., ::2]), dict(out=torch.zeros(5, 4, 16)), dict(out=torch.zeros(4, 4, 32)), dict(tree=torch.zeros(5, 1, dtype=i32)),
+    dict(tree=torch.zeros(4, 1, dtype=torch.int64)), dict(tree=torch.zeros(5, 0, dtype=torch.int64)), dict(tree=torch.zeros(2, 5, dtype=torch.int64).t())])
+def test_bad_attention_calls_are_refused(change):
+    with pytest.raises(ValueError, match="paged cache"):
+        _attend(**change)
+
+
+def test_bad_scores_are_refused():
+    x, y = torch.zeros(4, 9), torch.zeros(4, dtype=torch.int64)
+    for args, kw in (((x.half(), y), {}), ((x.double(), y), {}), ((x, y.int()), {}), ((x, y[:3]), {}), ((x, y), {"top": 10}), ((x, y), {"top": -1}),
+                     ((torch.zeros(4, 99), y), {"top": 65}), ((x, y), {"temperature": 0.0}), ((x, y), {"temperature": -1.0}),
+                     ((x, y), {"temperature": float("nan")}), ((x, y), {"temperature": float("inf")}), ((x,), {}), ((torch.zeros(4, 0), y), {}),
+                     ((torch.tensor(1.0), torch.tensor(0)), {})):
+        with pytest.raises(ValueError, match="token_logprobs"):
+            Fn.token_logprobs(*args, **kw)
+
+
+def test_the_c_entries_refuse_before_they_launch():
+    lib = L.lib()
+    assert lib.s2t_paged_kv_append(None, None) == -1 and lib.s2t_paged_attention(None, None) == -1
+    a = L.PagedArgs()
+    assert lib.s2t_paged_attention(C.byref(a), None) == -1
+    buf = torch.zeros(64, dtype=torch.float64)
+    p = buf.data_ptr()
+    p += -p % 16
+
+    def args(**change):
+        a = L.PagedArgs(dtype=0, B=1, N=0, max_new=1, q_heads=2, kv_heads=1, dk=32, num_pages=1, page_size=16, table_pages=1, k_pages=p, v_pages=p,
+                        p_sp=512, p_sh=512, p_sr=32, page_table=p, table_stride=1, lens=p, cu=p, k=p, k_st=32, k_sh=32, v=p, v_st=32, v_sh=32, q=p,
+                        q_st=64, q_sh=32, q_out=p, qo_st=64, qo_sh=32, out=p, o_st=64, o_sh=32, scale=1.0)
+        for k, v in change.items():
+            setattr(a, k, v)
+        return a
+
+    for entry in (lib.s2t_paged_kv_append, lib.s2t_paged_attention):
+        assert entry(C.byref(args()), None) == 0  # no rows: nothing is launched
+        for status, change in ((-2, dict(dtype=2)), (-1, dict(B=0)), (-1, dict(B=65536)), (-1, dict(page_size=24)), (-1, dict(q_heads=3, kv_heads=2)),
+                               (-4, dict(dk=24)), (-4, dict(dk=272)), (-1, dict(num_pages=0)), (-1, dict(lens=None)), (-3, dict(k_pages=p + 4)),
+                               (-3, dict(p_sr=33)), (-3, dict(q_st=66)), (-4, dict(table_pages=1 << 27))):
+            assert entry(C.byref(args(**change)), None) == status, change
+    assert lib.s2t_paged_kv_append(C.byref(args(rows=p)), None) == -1            # with q
+    assert lib.s2t_paged_kv_append(C.byref(args(rotary=p, rot_dim=48, rotary_positions=1)), None) == -1
+    assert lib.s2t_paged_attention(C.byref(args(tree=p, tree_words=0)), None) == -1
+    f, b = lib.s2t_token_logprobs_fwd, lib.s2t_token_logprobs_bwd
+    assert f(0, p, 8, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == 0
+    assert f(0, p, 7, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == -1       # rows overlap
+    assert f(2, p, 8, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == -2
+    assert f(0, p, 99, 0, 99, p, -1, 1.0, 65, p, p, p, p, p, None) == -4
+    assert f(0, p, 8, 1, 8, p, -1, 1.0, 2, p, p, p, None, p, None) == -1
+    assert f(0, p, 8, 1, 8, None, -1, 1.0, 0, p, p, p, None, None, None) == -1    # a score without a token
+    assert b(0, p, 8, 0, 8, p, -1, 1.0, 0, p, None, p, None, None, None, p, 8, None) == 0
+    assert b(0, p, 8, 1, 8, p, -1, 1.0, 0, p, None, p, p, None, None, p, 8, None) == -1   # g_entropy without the entropy
+    assert b(0, p, 8, 1, 8, p, -1, 1.0, 2, p, None, None, None, p, None, p, 8, None) == -1  # g_top without the columns
+
+
+def test_rotary_table():
+    t = M.rotary_table(5, 32)
+    assert t.shape == (5, 32) and torch.equal(t[0], torch.cat([torch.ones(16), torch.zeros(16)]))
+    far = M.rotary_table(100001, 32)[100000].double()
+    w = 10000.0 ** (-torch.arange(0, 32, 2, dtype=torch.float64) / 32)
+    assert float((far - torch.cat([torch.cos(1e5 * w), torch.sin(1e5 * w)])).abs().max()) < 2.0 ** -24
