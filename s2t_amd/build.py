@@ -20,7 +20,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-res
 # every one of them out again for the softmax arithmetic (64 v_accvgpr moves per 16 x 64 step in kernels that are bound by
 # vector issue); with the results in ordinary VGPRs the copies are gone and the kernels need FEWER registers (dQ 224 -> 208,
 # the decoder's dK/dV 180 -> 168): dQ 44.1 -> 43.3 us, dK/dV 46.6 -> 44.4 us per launch on MI355X.
-FILE_FLAGS = {"attention_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# paged.hip: the same (one tile row of 64-wide bf16 heads: 172 -> 148 registers, three waves of a SIMD instead of two).
+FILE_FLAGS = {"attention_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _sources():

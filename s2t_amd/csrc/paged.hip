@@ -1,5 +1,7 @@
 // Paged key/value cache of an incremental decoder: append (with rotary positions on the way) and attention of several new tokens of a
 // sequence over it, chain or tree of drafts.  Layout, bounds and semantics: include/s2t_hip.h, s2t_paged_args.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -86,55 +88,510 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 }
 
 // ---- attention --------------------------------------------------------------------------------------------------------------
-// One wave per (new token, query head): a lane scores one key of each 64, the running maximum and sum are the wave's, and every lane
-// keeps dk / 64 columns of the output.
-template <typename T>
-__global__ __launch_bounds__(64) void paged_attention_kernel(const s2t_paged_args a, int shift) {
-  const int b = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x;
-  const Span s = span_of(a, b);
-  if (i >= s.n) return;
-  const int t = s.row0 + i, prefix = s.len - s.n;
-  const int64_t kvh = (int64_t)(h / (a.q_heads / a.kv_heads)) * a.p_sh;
-  const Pages pg = pages_of(a, shift, b);
-  const int len = (int)min((int64_t)s.len, (int64_t)a.table_pages << shift);
-  __shared__ float qs[256];
-  for (int c = lane; c < a.dk; c += 64) qs[c] = ld_as_f32<T>((const T*)a.q + t * a.q_st + h * a.q_sh + c) * a.scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < len; k0 += 64) {
-    const int key = k0 + lane, j = key - prefix;
-    bool sees = key < len;
-    if (j >= 0) {
-      if (a.tree) sees = sees && j < 64 * a.tree_words && ((a.tree[t * a.tree_stride + (j >> 6)] >> (j & 63)) & 1);
-      else sees = sees && j <= i;
-    }
-    const int64_t at = sees ? pg.at(key) : -1;
-    float sc = -INFINITY;
-    if (at >= 0) {
-      const T* kr = (const T*)a.k_pages + at + kvh;
-      sc = 0.f;
-      for (int c = 0; c < a.dk; ++c) sc += qs[c] * ld_as_f32<T>(kr + c);
-    }
-    const float mn = fmaxf(m, wave_max(sc)), ref = mn == -INFINITY ? 0.f : mn;
-    const float p = at >= 0 ? __expf(sc - ref) : 0.f, fade = __expf(m - ref);
-    m = mn;
-    l = l * fade + wave_sum(p);
+// A workgroup takes 16 * MT rows (new token x query head of one key/value head's group) and a range of keys, its four waves every
+// fourth tile of 32 keys; their results meet in LDS, those of several ranges in paged_combine_kernel.  Nothing but that goes through LDS:
+// the products are laid out so that what a matrix instruction returns is what the next one takes, and K and V go from the pages to
+// its operands by plain 16-byte loads.
+//   S^T = K Q^T      A: lane (c, g) holds key c of a half tile, 8 (fp32: 4) elements; it returns lane (c, g) query c, keys 4g .. 4g + 3
+//   O^T += V^T P^T   B: lane (c, g) holds query c, its 8 keys 4g .. 4g + 3 of both halves: those; the keys of A in the same order.
+//                    A: lane (c, g) loads columns c * NDT .. of its 8 keys, 16 lanes a whole row, and (bf16) pairs keys by v_perm.
+// Scores, running reference and sums are fp32, in powers of two.  The reference of a row moves only when a score passes it by 2^8
+// (a vote; no exchange between lanes otherwise), so p < 2^8.  bf16 P is held as two bf16 numbers (2^-16 of the value): one rounding to
+// bf16 would add an error as large as the output's own.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int MIN_CHUNK = 256;  // keys of a range: two tiles for each wave
+
+__device__ __forceinline__ bool finite_(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// keys of each of n_split ranges of a row tile that sees keys 0 .. kend - 1
+__device__ __forceinline__ int chunk_of(int kend, int n_split) {
+  return max(MIN_CHUNK, ((kend + n_split - 1) / n_split + 127) & ~127);
+}
+__device__ __forceinline__ int ranges_of(int kend, int chunk) { return max(1, (kend + chunk - 1) / chunk); }
+
+// what a row tile sees: rows of this launch, first key after the last that any of its rows may see
+struct Reach {
+  int rows, len, prefix, kend;
+};
+__device__ __forceinline__ Reach reach_of(const s2t_paged_args& a, const Span& s, int shift, int group, int row_base, int tile_rows) {
+  Reach r;
+  r.rows = min(s.n, a.max_new) * group;
+  r.len = min(s.len, a.table_pages << shift);
+  r.prefix = s.len - s.n;
+  const int last = (min(row_base + tile_rows, r.rows) - 1) / group;
+  r.kend = a.tree ? r.len : min(r.len, r.prefix + last + 1);
+  return r;
+}
+
+// bits of new tokens j0 .. j0 + 31 (bits of tokens below 0 are clear)
+__device__ __forceinline__ uint32_t tree_window(const int64_t* __restrict__ row, int words, int j0) {
+  const int lo = j0 >> 6, sh = j0 & 63;
+  const uint64_t x = (uint32_t)lo < (uint32_t)words ? (uint64_t)row[lo] : 0, y = (uint32_t)(lo + 1) < (uint32_t)words ? (uint64_t)row[lo + 1] : 0;
+  return (uint32_t)((x >> sh) | (sh ? y << (64 - sh) : 0));
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// T: type of the cache; DK: head_dim rounded up to 32, 64, 128 or 256; BIG: a half tile of 16 keys lies in one page
+template <typename T, int DK, int MT, bool BIG>
+__global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int n_tiles, const int n_split,
+                                                              const float c2, const int flip, float* __restrict__ part) {
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int NDT = DK / 16;          // 16-column tiles of the output
+  constexpr int KE = BF ? 8 : 4;        // elements of 16 bytes
+  constexpr int NK = DK / (4 * KE);     // 16-byte loads of a key
+  constexpr int VB = NDT * (int)sizeof(T);  // bytes that a lane loads of a value row
+  __shared__ float obuf[4][MT][4][64][NDT];
+  __shared__ float mlbuf[4][MT][16][2];
+
+  // all row tiles and ranges of a (sequence, key/value head) on one XCD (workgroups go round the eight), the longest tiles first
+  const int per = n_tiles * n_split, slot = blockIdx.x >> 3;
+  const int pair = (slot / per) * 8 + (blockIdx.x & 7), unit = slot % per;
+  if (pair >= a.B * a.kv_heads) return;
+  const int b = pair / a.kv_heads, h = pair % a.kv_heads;
+  const int split = unit % n_split, row_base = (n_tiles - 1 - unit / n_split) * 16 * MT;
+  const int group = a.q_heads / a.kv_heads;
+  const Span sp = span_of(a, b);
+  const Reach rc = reach_of(a, sp, shift, group, row_base, 16 * MT);
+  if (row_base >= rc.rows) return;
+  const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
+  if (split >= used) return;
+  const int k_hi = min(rc.kend, (split + 1) * chunk);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int d = a.dk;
+  const T* kpool = (const T*)a.k_pages + h * a.p_sh;
+  const T* vpool = (const T*)a.v_pages + h * a.p_sh;
+  const int32_t* table = a.page_table + b * a.table_stride;
+  const int sr = (int)a.p_sr, mask = a.page_size - 1;
+
+  // queries: operand B of S^T
+  u32x4 qf[MT][NK];
+  int tok[MT];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] *= fade;
-    for (int u = 0; u < 64; ++u) {
-      const int64_t au = __shfl(at, u, 64);
-      if (au < 0) continue;
-      const float pu = __shfl(p, u, 64);
+  for (int mt = 0; mt < MT; ++mt) {
+    const int row = row_base + mt * 16 + c;
+    const bool live = row < rc.rows;
+    tok[mt] = live ? row / group : 0;
+    const T* q = (const T*)a.q + (int64_t)(sp.row0 + tok[mt]) * a.q_st + (int64_t)(h * group + (live ? row % group : 0)) * a.q_sh;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r * 64 + lane < a.dk) o[r] += pu * ld_as_f32<T>((const T*)a.v_pages + au + kvh + r * 64 + lane);
+    for (int ks = 0; ks < NK; ++ks) {
+      const int col = (ks * 4 + g) * KE;
+      u32x4 v = {0, 0, 0, 0};
+      if (live && col < d) v = *reinterpret_cast<const u32x4*>(q + col);
+      if (flip) v ^= BF ? 0x80008000u : 0x80000000u;  // a negative scale
+      qf[mt][ks] = v;
     }
   }
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+
+  f32x4 acc[MT][NDT];
+  float m[MT], l[MT];
+  const int vcol = min(c * NDT, d - NDT);  // padded columns repeat the last ones; they are not written
+
+  // where 32 keys lie: the two half tiles' first keys (BIG), or this lane's key
+  struct Where {
+    int64_t half0, half1;  // BIG
+    int64_t row;           // !BIG: offset of key key0 + (lane & 31)
+    uint32_t exist;        // bit of each of the 32 keys: it lies on a page
+  };
+  auto find = [&](int key0) {
+    Where w;
+    if constexpr (BIG) {
+      const int i0 = key0 >> shift, i1 = (key0 + 16) >> shift;
+      const int p0 = i0 < a.table_pages ? table[i0] : -1, p1 = i1 < a.table_pages ? table[i1] : -1;
+      const bool ok0 = (uint32_t)p0 < (uint32_t)a.num_pages, ok1 = (uint32_t)p1 < (uint32_t)a.num_pages;
+      w.half0 = (ok0 ? p0 * a.p_sp : 0) + (int64_t)(key0 & mask) * sr;
+      w.half1 = (ok1 ? p1 * a.p_sp : 0) + (int64_t)((key0 + 16) & mask) * sr;
+      w.exist = (ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u);
+    } else {
+      const int key = key0 + (lane & 31), i = key >> shift;
+      const int p = i < a.table_pages ? table[i] : -1;
+      const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
+      w.row = ok ? p * a.p_sp + (int64_t)(key & mask) * sr : 0;
+      w.exist = (uint32_t)__ballot(ok);
+    }
+    return w;
+  };
+  // (BIG: a scalar base and one 32-bit offset of the lane for all loads of a tile)
+  const uint32_t koff = (uint32_t)(c * sr) * (uint32_t)sizeof(T), voff = (uint32_t)(4 * g * sr + vcol) * (uint32_t)sizeof(T);
+  auto load_k = [&](const Where& w, u32x4 (&kf)[2][NK]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (r * 64 + lane < a.dk) st_from_f32<T>((T*)a.out + t * a.o_st + h * a.o_sh + r * 64 + lane, m == -INFINITY ? 0.f : o[r] * inv);
-  if (a.lse && lane == 0) a.lse[(int64_t)t * a.q_heads + h] = m == -INFINITY ? -INFINITY : m + __logf(l);
+    for (int t = 0; t < 2; ++t) {
+      const char* p;
+      if constexpr (BIG) p = (const char*)(kpool + (t ? w.half1 : w.half0)) + koff;
+      else p = (const char*)(kpool + (int64_t)__shfl(w.row, 16 * t + c, 64));
+#pragma unroll
+      for (int ks = 0; ks < NK; ++ks) kf[t][ks] = *reinterpret_cast<const u32x4*>(p + (uint32_t)min((ks * 4 + g) * KE, d - KE) * (uint32_t)sizeof(T));
+    }
+    if (d != DK) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks)
+          if ((ks * 4 + g) * KE >= d) kf[t][ks] = u32x4{0, 0, 0, 0};
+    }
+  };
+  constexpr int VW = VB / 4;  // dwords of a lane's piece of a value row
+  auto load_v = [&](const Where& w, uint32_t (&vr)[8][VW]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const char* p;
+      if constexpr (BIG) p = (const char*)(vpool + (e >> 2 ? w.half1 : w.half0) + (e & 3) * sr) + voff;
+      else p = (const char*)(vpool + vcol + (int64_t)__shfl(w.row, 16 * (e >> 2) + 4 * g + (e & 3), 64));
+      if constexpr (VB == 4) vr[e][0] = *reinterpret_cast<const uint32_t*>(p);
+      else if constexpr (VB == 8) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        vr[e][0] = x.x;
+        vr[e][1] = x.y;
+      } else {
+#pragma unroll
+        for (int q = 0; q < VW / 4; ++q) {
+          const u32x4 x = reinterpret_cast<const u32x4*>(p)[q];
+          vr[e][4 * q] = x.x;
+          vr[e][4 * q + 1] = x.y;
+          vr[e][4 * q + 2] = x.z;
+          vr[e][4 * q + 3] = x.w;
+        }
+      }
+    }
+  };
+
+  // The first time round trusts the values that are seen: a 0 times infinity or NaN (a value that some rows of the tile do not see, or a
+  // low half of p) leaves a result that is not finite.  Then the wave goes over its keys once more, taking those values out of the
+  // matrix product and adding them to the rows that see them.
+  auto go = [&](auto again) {
+    constexpr bool careful = decltype(again)::value;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt] = -INFINITY;
+      l[mt] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    u32x4 kf[2][NK];
+    int key0 = split * chunk + 32 * wave;
+    Where w;
+    if (key0 < k_hi) {
+      w = find(key0);
+      load_k(w, kf);
+    }
+    while (key0 < k_hi) {
+      uint32_t vr[8][VW];
+      load_v(w, vr);
+      // scores of all rows, then the next tile's keys can be fetched
+      f32x4 s[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < NK; ++ks) {
+            if constexpr (BF)
+              x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[t][ks]), __builtin_bit_cast(bf16x8, qf[mt][ks]), x, 0, 0, 0);
+            else
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][ks][e]), __uint_as_float(qf[mt][ks][e]), x, 0, 0, 0);
+          }
+          s[mt][t] = x;
+        }
+      const Where now = w;
+      const int next = key0 + 128;
+      if (next < k_hi) {
+        w = find(next);
+        load_k(w, kf);
+      }
+      // keys of this tile that exist, and whether every row sees all of them
+      const uint32_t exist = low_bits(rc.len - key0) & now.exist;
+      const bool whole = exist == 0xffffffffu && key0 + 32 <= rc.prefix;
+      uint32_t vis[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        vis[mt] = 0xffffffffu;
+        if (!whole) {
+          const int j0 = key0 - rc.prefix;
+          uint32_t x;
+          if (a.tree) x = tree_window(a.tree + (int64_t)(sp.row0 + tok[mt]) * a.tree_stride, a.tree_words, j0) | low_bits(-j0);
+          else x = low_bits(tok[mt] - j0 + 1);
+          vis[mt] = x & exist;
+          const uint32_t mine = vis[mt] >> (4 * g);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!((mine >> (16 * t + r)) & 1)) s[mt][t][r] = -INFINITY;
+        }
+        // reference
+        const float top = c2 * fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                                     fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
+        if (__any(top > m[mt] + 8.f)) {
+          const float mn = fmaxf(m[mt], s2t_xmax<16>(s2t_xmax<32>(top)));
+          const float fade = mn == -INFINITY ? 1.f : exp2_(m[mt] - mn);
+          m[mt] = mn;
+          l[mt] *= fade;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] *= fade;
+        }
+      }
+      // values: operand A of O^T
+      if (exist != 0xffffffffu) {  // what lies behind the end is not to be multiplied with anything
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!((exist >> (16 * (e >> 2) + 4 * g + (e & 3))) & 1))
+#pragma unroll
+            for (int q = 0; q < VW; ++q) vr[e][q] = 0;
+      }
+      if constexpr (careful) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int q = 0; q < VW; ++q) {
+            if constexpr (BF) {
+              if ((vr[e][q] & 0x7f80u) == 0x7f80u) vr[e][q] &= 0xffff0000u;
+              if ((vr[e][q] & 0x7f800000u) == 0x7f800000u) vr[e][q] &= 0xffffu;
+            } else if (!finite_(__uint_as_float(vr[e][q]))) vr[e][q] = 0;
+          }
+      }
+      u32x4 va[BF ? NDT : 1];
+      if constexpr (BF) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            va[dt][q] = __builtin_amdgcn_perm(vr[2 * q + 1][dt >> 1], vr[2 * q][dt >> 1], dt & 1 ? 0x07060302u : 0x05040100u);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+        float p[2][4], sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[t][r] = exp2_(fmaf(s[mt][t][r], c2, -ref));
+            sum += p[t][r];
+          }
+        l[mt] += sum;
+        if constexpr (BF) {
+          u32x4 hi, lo;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float x = p[q >> 1][2 * (q & 1)], y = p[q >> 1][2 * (q & 1) + 1];
+            hi[q] = bf16pack(x, y);
+            lo[q] = bf16pack(x - __uint_as_float(hi[q] << 16), y - __uint_as_float(hi[q] & 0xffff0000u));
+          }
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) {
+            acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va[dt]), __builtin_bit_cast(bf16x8, hi), acc[mt][dt], 0, 0, 0);
+            acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va[dt]), __builtin_bit_cast(bf16x8, lo), acc[mt][dt], 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int dt = 0; dt < NDT; ++dt)
+                acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + r][dt]), p[t][r], acc[mt][dt], 0, 0, 0);
+        }
+        if constexpr (careful) {
+          float* seen = &obuf[wave][0][0][0][0];  // [key][query]: p, -1 where the row does not see the key (obuf is free until the end)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) seen[(16 * t + 4 * g + r) * 16 + c] = (vis[mt] >> (16 * t + 4 * g + r)) & 1 ? p[t][r] : -1.f;
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+          for (int key = 0; key < 32; ++key) {
+            if (!((exist >> key) & 1)) continue;
+            int64_t at;
+            if constexpr (BIG) at = (key >> 4 ? now.half1 : now.half0) + (key & 15) * sr;
+            else at = (int64_t)__shfl(now.row, key, 64);
+            const float pk = seen[key * 16 + c];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int dt = 0; dt < NDT; ++dt) {
+                const float v = ld_as_f32<T>(vpool + at + min((4 * g + r) * NDT + dt, d - 1));
+                if (!(pk < 0.f) && !finite_(v)) acc[mt][dt][r] += pk * v;
+              }
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      key0 = next;
+    }
+  };
+  go(std::false_type{});
+  float sick = 0.f;  // a sum of 0 * x: 0, or NaN if any x is not finite
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sick = fmaf(acc[mt][dt][r], 0.f, sick);
+  if (__any(sick != sick)) go(std::true_type{});
+
+  // the four waves' results; wave w then finishes rows 4g + w of every 16 columns
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l[mt] = s2t_xadd<16>(s2t_xadd<32>(l[mt]));
+    if (g == 0) {
+      mlbuf[wave][mt][c][0] = m[mt];
+      mlbuf[wave][mt][c][1] = l[mt];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) obuf[wave][mt][r][lane][dt] = acc[mt][dt][r];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    float mw[4], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mw[w] = mlbuf[w][mt][c][0];
+      top = fmaxf(top, mw[w]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top;
+    float total = 0.f, o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2_(mw[w] - ref);
+      total += f * mlbuf[w][mt][c][1];
+      if (mw[w] != -INFINITY)
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] += f * obuf[w][mt][wave][lane][dt];
+    }
+    const int row = row_base + mt * 16 + c, col = (4 * g + wave) * NDT;
+    if (row >= rc.rows || col >= d) continue;
+    const int t = sp.row0 + row / group, hq = h * group + row % group;
+    if (used == 1) {
+      const float inv = top == -INFINITY ? 0.f : 1.f / total;
+      T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt += 2) {
+        if constexpr (BF) *reinterpret_cast<uint32_t*>(out + dt) = bf16pack(o[dt] * inv, o[dt + 1] * inv);
+        else {
+          out[dt] = o[dt] * inv;
+          out[dt + 1] = o[dt + 1] * inv;
+        }
+      }
+      if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
+    } else {  // part: [split][token][query head][d + 2]
+      float* to = part + (((int64_t)split * a.N + t) * a.q_heads + hq) * (d + 2);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) to[col + dt] = o[dt];
+      if (col == 0) {
+        to[d] = top;
+        to[d + 1] = total;
+      }
+    }
+  }
+}
+
+// Joins the ranges of one (new token, query head): weights 2^(m - max m), in the order of the ranges.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args a, const int shift, const int tile_rows, const int n_split,
+                                                            const float* __restrict__ part) {
+  __shared__ float weight[256];
+  __shared__ float sum[4][256];
+  const int b = blockIdx.y, i = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads;
+  const int group = a.q_heads / a.kv_heads, d = a.dk;
+  const Span sp = span_of(a, b);
+  if (i >= min(sp.n, a.max_new)) return;
+  const Reach rc = reach_of(a, sp, shift, group, (i * group + hq % group) / tile_rows * tile_rows, tile_rows);
+  const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
+  if (used == 1) return;
+  const int64_t t = sp.row0 + i, step = (int64_t)a.N * a.q_heads * (d + 2);
+  const float* p = part + (t * a.q_heads + hq) * (d + 2);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  float top = -INFINITY;
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, p[s * step + d]);
+  top = wave_max(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  for (int s = lane; s < used; s += 64) {
+    const float f = exp2_(p[s * step + d] - ref);
+    total += f * p[s * step + d + 1];
+    if (w == 0) weight[s] = f;
+  }
+  total = wave_sum(total);
+  __syncthreads();
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = w; s < used; s += 4) {
+    const float f = weight[s];
+    if (f == 0.f && p[s * step + d] == -INFINITY) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 64 + lane < d) o[q] += f * p[s * step + q * 64 + lane];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sum[w][q * 64 + lane] = o[q];
+  __syncthreads();
+  if (tid < d) {
+    const float x = ((sum[0][tid] + sum[1][tid]) + sum[2][tid]) + sum[3][tid];
+    st_from_f32<T>((T*)a.out + t * a.o_st + hq * a.o_sh + tid, top == -INFINITY ? 0.f : x / total);
+  }
+  if (a.lse && tid == 0) a.lse[t * a.q_heads + hq] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
+}
+
+// How a call is cut: rows of a tile, tiles of a sequence, ranges of the keys.
+struct Cut {
+  int mt, tiles, splits;
+};
+Cut cut_of(const s2t_paged_args* a) {
+  const int64_t rows = (int64_t)a->max_new * (a->q_heads / a->kv_heads);
+  const int most = a->dk <= 64 ? 4 : a->dk <= 128 ? 2 : 1;
+  Cut c;
+  c.mt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  c.tiles = (int)((rows + 16 * c.mt - 1) / (16 * c.mt));
+  const int64_t units = (int64_t)c.tiles * a->kv_heads * a->B, keys = (int64_t)a->table_pages * a->page_size;
+  int64_t s = (2048 + units - 1) / units;
+  const int64_t can = (keys + MIN_CHUNK - 1) / MIN_CHUNK;
+  if (s > can) s = can;
+  if (s > 256) s = 256;
+  c.splits = (int)s;
+  return c;
+}
+
+template <typename T, int DK, int MT>
+void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
+  const int64_t pairs = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8;
+  const dim3 grid((unsigned)(pairs * c.tiles * c.splits));
+  const int shift = __builtin_ctz((unsigned)a->page_size), flip = a->scale < 0.f;
+  const float c2 = fmaxf(fabsf(a->scale) * LOG2E, 1e-30f);  // never 0: 0 times the -inf of a hidden key is not 0
+  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
+}
+template <typename T>
+void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
+  if (a->dk <= 32) {
+    if (c.mt == 1) launch_attention<T, 32, 1>(a, c, st);
+    else if (c.mt == 2) launch_attention<T, 32, 2>(a, c, st);
+    else launch_attention<T, 32, 4>(a, c, st);
+  } else if (a->dk <= 64) {
+    if (c.mt == 1) launch_attention<T, 64, 1>(a, c, st);
+    else if (c.mt == 2) launch_attention<T, 64, 2>(a, c, st);
+    else launch_attention<T, 64, 4>(a, c, st);
+  } else if (a->dk <= 128) {
+    if (c.mt == 1) launch_attention<T, 128, 1>(a, c, st);
+    else launch_attention<T, 128, 2>(a, c, st);
+  } else {
+    launch_attention<T, 256, 1>(a, c, st);
+  }
+  if (c.splits > 1)
+    hipLaunchKernelGGL(paged_combine_kernel<T>, dim3((unsigned)(a->max_new * a->q_heads), (unsigned)a->B), dim3(256), 0, st, *a,
+                       __builtin_ctz((unsigned)a->page_size), 16 * c.mt, c.splits, (const float*)a->ws);
 }
 
 int paged_args_bad(const s2t_paged_args* a) {
@@ -170,18 +627,27 @@ extern "C" int s2t_paged_kv_append(const s2t_paged_args* a, void* stream) {
   return S2T_LAUNCH_CHECK();
 }
 
-extern "C" int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* a) { return paged_args_bad(a) ? -1 : 0; }
+extern "C" int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* a) {
+  if (paged_args_bad(a)) return -1;
+  if (a->N == 0 || a->max_new == 0) return 0;
+  const Cut c = cut_of(a);
+  return c.splits > 1 ? (int64_t)c.splits * a->N * a->q_heads * (a->dk + 2) * 4 : 0;
+}
 
 extern "C" int s2t_paged_attention(const s2t_paged_args* a, void* stream) {
   if (int bad = paged_args_bad(a)) return bad;
-  if ((a->tree && a->tree_words <= 0) || a->q_heads > 65535) return S2T_ERR_ARG;
+  if ((a->tree && a->tree_words <= 0) || !(a->scale == a->scale)) return S2T_ERR_ARG;
   if (misaligned(a, a->k_pages, a->p_sp, a->p_sh) || misaligned(a, a->v_pages, a->p_sr, 0) || misaligned(a, a->q, a->q_st, a->q_sh) ||
       misaligned(a, a->out, a->o_st, a->o_sh) || ((uintptr_t)a->tree & 7))
     return S2T_ERR_ALIGN;
   if (a->N == 0 || a->max_new == 0) return S2T_OK;
   if (!a->q || !a->out) return S2T_ERR_ARG;
-  const dim3 grid((unsigned)a->max_new, (unsigned)a->q_heads, (unsigned)a->B);
-  if (a->dtype == S2T_F32) hipLaunchKernelGGL(paged_attention_kernel<float>, grid, dim3(64), 0, (hipStream_t)stream, *a, shift_of(a));
-  else hipLaunchKernelGGL(paged_attention_kernel<bf16_t>, grid, dim3(64), 0, (hipStream_t)stream, *a, shift_of(a));
+  const Cut c = cut_of(a);
+  const int64_t blocks = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8 * c.tiles * c.splits;
+  // launch bounds, and 32-bit offsets of the 16 rows of a half tile
+  if (blocks > 0x7fffffff || (int64_t)a->max_new * a->q_heads > 0x7fffffff || a->p_sr < 0 || a->p_sr > (1 << 24)) return S2T_ERR_UNSUPPORTED;
+  if (c.splits > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < s2t_paged_attention_ws_bytes(a))) return S2T_ERR_ARG;
+  if (a->dtype == S2T_F32) launch_attention<float>(a, c, (hipStream_t)stream);
+  else launch_attention<bf16_t>(a, c, (hipStream_t)stream);
   return S2T_LAUNCH_CHECK();
 }
