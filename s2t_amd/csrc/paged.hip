@@ -102,7 +102,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int MIN_CHUNK = 256;  // keys of a range: two tiles for each wave
+constexpr int MIN_CHUNK = 512;  // keys of a range: four tiles for each wave
 
 __device__ __forceinline__ bool finite_(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -147,10 +147,18 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   __shared__ float obuf[4][MT][4][64][NDT];
   __shared__ float mlbuf[4][MT][16][2];
 
-  // all row tiles and ranges of a (sequence, key/value head) on one XCD (workgroups go round the eight), the longest tiles first
-  const int per = n_tiles * n_split, slot = blockIdx.x >> 3;
-  const int pair = (slot / per) * 8 + (blockIdx.x & 7), unit = slot % per;
-  if (pair >= a.B * a.kv_heads) return;
+  // all row tiles of a (sequence, key/value head) on one XCD (workgroups go round the eight), the longest tiles first
+  const int per = n_tiles * n_split, pairs = a.B * a.kv_heads;
+  int pair, unit;
+  if (n_tiles > 1 && pairs >= 8) {
+    const int slot = blockIdx.x >> 3;
+    pair = (slot / per) * 8 + (blockIdx.x & 7);
+    unit = slot % per;
+  } else {
+    pair = blockIdx.x % pairs;
+    unit = blockIdx.x / pairs;
+  }
+  if (pair >= pairs || unit >= per) return;
   const int b = pair / a.kv_heads, h = pair % a.kv_heads;
   const int split = unit % n_split, row_base = (n_tiles - 1 - unit / n_split) * 16 * MT;
   const int group = a.q_heads / a.kv_heads;
@@ -160,6 +168,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
   if (split >= used) return;
   const int k_hi = min(rc.kend, (split + 1) * chunk);
+  const int all_see = rc.prefix + (a.tree ? 0 : row_base / group + 1);  // every row of the tile sees the keys before this one
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -201,8 +210,10 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   auto find = [&](int key0) {
     Where w;
     if constexpr (BIG) {
+      // (the table through scalar loads: as vector loads they would wait behind the values that are on their way)
+      const auto entries = (const __attribute__((address_space(4))) int32_t*)table;
       const int i0 = key0 >> shift, i1 = (key0 + 16) >> shift;
-      const int p0 = i0 < a.table_pages ? table[i0] : -1, p1 = i1 < a.table_pages ? table[i1] : -1;
+      const int p0 = i0 < a.table_pages ? entries[i0] : -1, p1 = i1 < a.table_pages ? entries[i1] : -1;
       const bool ok0 = (uint32_t)p0 < (uint32_t)a.num_pages, ok1 = (uint32_t)p1 < (uint32_t)a.num_pages;
       w.half0 = (ok0 ? p0 * a.p_sp : 0) + (int64_t)(key0 & mask) * sr;
       w.half1 = (ok1 ? p1 * a.p_sp : 0) + (int64_t)((key0 + 16) & mask) * sr;
@@ -263,6 +274,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   // The first time round trusts the values that are seen: a 0 times infinity or NaN (a value that some rows of the tile do not see, or a
   // low half of p) leaves a result that is not finite.  Then the wave goes over its keys once more, taking those values out of the
   // matrix product and adding them to the rows that see them.
+  float* seen = &obuf[wave][0][0][0][0];  // that round's [row tile][key][query]: p, -1 where the row does not see the key (obuf is free until the end)
   auto go = [&](auto again) {
     constexpr bool careful = decltype(again)::value;
 #pragma unroll
@@ -275,13 +287,17 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
     u32x4 kf[2][NK];
     int key0 = split * chunk + 32 * wave;
     Where w;
-    if (key0 < k_hi) {
+    uint32_t vr[8][VW];
+    if (!careful && key0 < k_hi) {
       w = find(key0);
       load_k(w, kf);
-    }
-    while (key0 < k_hi) {
-      uint32_t vr[8][VW];
       load_v(w, vr);
+    }
+    while (key0 < k_hi) {  // (a tile's keys and values are both on their way while the tile before it is worked on)
+      if constexpr (careful) {  // (with nothing on its way, and the corrections last: this round is not to need more registers)
+        w = find(key0);
+        load_k(w, kf);
+      }
       // scores of all rows, then the next tile's keys can be fetched
       f32x4 s[MT][2];
 #pragma unroll
@@ -302,13 +318,15 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
         }
       const Where now = w;
       const int next = key0 + 128;
-      if (next < k_hi) {
+      if constexpr (careful) load_v(now, vr);
+      else if (next < k_hi) {
         w = find(next);
         load_k(w, kf);
       }
+      __builtin_amdgcn_sched_barrier(0);
       // keys of this tile that exist, and whether every row sees all of them
       const uint32_t exist = low_bits(rc.len - key0) & now.exist;
-      const bool whole = exist == 0xffffffffu && key0 + 32 <= rc.prefix;
+      const bool whole = exist == 0xffffffffu && key0 + 32 <= all_see;
       uint32_t vis[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -364,6 +382,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             va[dt][q] = __builtin_amdgcn_perm(vr[2 * q + 1][dt >> 1], vr[2 * q][dt >> 1], dt & 1 ? 0x07060302u : 0x05040100u);
+        if (!careful && next < k_hi) load_v(w, vr);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -400,31 +420,39 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
                 acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + r][dt]), p[t][r], acc[mt][dt], 0, 0, 0);
         }
         if constexpr (careful) {
-          float* seen = &obuf[wave][0][0][0][0];  // [key][query]: p, -1 where the row does not see the key (obuf is free until the end)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) seen[(16 * t + 4 * g + r) * 16 + c] = (vis[mt] >> (16 * t + 4 * g + r)) & 1 ? p[t][r] : -1.f;
-          __builtin_amdgcn_wave_barrier();
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-          for (int key = 0; key < 32; ++key) {
-            if (!((exist >> key) & 1)) continue;
-            int64_t at;
-            if constexpr (BIG) at = (key >> 4 ? now.half1 : now.half0) + (key & 15) * sr;
-            else at = (int64_t)__shfl(now.row, key, 64);
-            const float pk = seen[key * 16 + c];
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int dt = 0; dt < NDT; ++dt) {
-                const float v = ld_as_f32<T>(vpool + at + min((4 * g + r) * NDT + dt, d - 1));
-                if (!(pk < 0.f) && !finite_(v)) acc[mt][dt][r] += pk * v;
-              }
-          }
-          __builtin_amdgcn_wave_barrier();
+            for (int r = 0; r < 4; ++r) seen[(mt * 32 + 16 * t + 4 * g + r) * 16 + c] = (vis[mt] >> (16 * t + 4 * g + r)) & 1 ? p[t][r] : -1.f;
         }
       }
+      if constexpr (careful) {
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+          int64_t at = 0;
+          if constexpr (!BIG) at = (int64_t)__shfl(now.row, key, 64);
+          if (!((exist >> key) & 1)) continue;
+          if constexpr (BIG) at = (key >> 4 ? now.half1 : now.half0) + (key & 15) * sr;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+              const float v = ld_as_f32<T>(vpool + at + min((4 * g + r) * NDT + dt, d - 1));
+              if (!finite_(v))
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  const float pk = seen[(mt * 32 + key) * 16 + c];
+                  if (!(pk < 0.f)) acc[mt][dt][r] += pk * v;
+                }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      if constexpr (!BF && !careful)
+        if (next < k_hi) load_v(w, vr);
       key0 = next;
     }
   };
@@ -487,62 +515,73 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
         }
       }
       if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
-    } else {  // part: [split][token][query head][d + 2]
-      float* to = part + (((int64_t)split * a.N + t) * a.q_heads + hq) * (d + 2);
+    } else {  // part: [split][token][query head][d], then their [2]: reference and sum
+      const int64_t heads = (int64_t)a.N * a.q_heads, at = split * heads + (int64_t)t * a.q_heads + hq;
+      float* to = part + at * d + col;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) to[col + dt] = o[dt];
-      if (col == 0) {
-        to[d] = top;
-        to[d + 1] = total;
-      }
+      for (int dt = 0; dt < NDT; dt += 2) *reinterpret_cast<float2*>(to + dt) = make_float2(o[dt], o[dt + 1]);
+      if (col == 0) reinterpret_cast<float2*>(part + n_split * heads * d)[at] = make_float2(top, total);
     }
   }
 }
 
-// Joins the ranges of one (new token, query head): weights 2^(m - max m), in the order of the ranges.
-template <typename T>
+// Joins the ranges of the (new token, query head) rows, weights 2^(m - max m): WAVES waves to a row, `lanes` (a power of two) of them to a
+// range's columns, so that 64 * WAVES / lanes ranges are on their way at a time; the order of every sum is fixed.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args a, const int shift, const int tile_rows, const int n_split,
-                                                            const float* __restrict__ part) {
-  __shared__ float weight[256];
-  __shared__ float sum[4][256];
-  const int b = blockIdx.y, i = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads;
-  const int group = a.q_heads / a.kv_heads, d = a.dk;
+                                                            const int lanes, const float* __restrict__ part) {
+  __shared__ float sums[4][256];
+  const int b = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6, sub = WAVES == 1 ? 0 : w;
+  const int rowid = WAVES == 1 ? blockIdx.x * 4 + w : blockIdx.x;
+  const int i = rowid / a.q_heads, hq = rowid % a.q_heads, group = a.q_heads / a.kv_heads, d = a.dk;
   const Span sp = span_of(a, b);
-  if (i >= min(sp.n, a.max_new)) return;
+  const bool live = i < min(sp.n, a.max_new);
   const Reach rc = reach_of(a, sp, shift, group, (i * group + hq % group) / tile_rows * tile_rows, tile_rows);
   const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
-  if (used == 1) return;
-  const int64_t t = sp.row0 + i, step = (int64_t)a.N * a.q_heads * (d + 2);
-  const float* p = part + (t * a.q_heads + hq) * (d + 2);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (!live || used == 1) return;  // (WAVES == 4: the whole workgroup)
+  const int64_t heads = (int64_t)a.N * a.q_heads, t = sp.row0 + i, at = t * a.q_heads + hq;
+  const float2* ml = reinterpret_cast<const float2*>(part + n_split * heads * d) + at;
   float top = -INFINITY;
-  for (int s = lane; s < used; s += 64) top = fmaxf(top, p[s * step + d]);
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, ml[s * heads].x);
   top = wave_max(top);
   const float ref = top == -INFINITY ? 0.f : top;
+  const int col = (lane & (lanes - 1)) * 4, first = sub * (64 / lanes) + lane / lanes, step = WAVES * (64 / lanes);
   float total = 0.f;
-  for (int s = lane; s < used; s += 64) {
-    const float f = exp2_(p[s * step + d] - ref);
-    total += f * p[s * step + d + 1];
-    if (w == 0) weight[s] = f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = first; s < used; s += step) {
+    const float2 x = ml[s * heads];
+    const float f = exp2_(x.x - ref);
+    const f32x4 y = col < d ? *reinterpret_cast<const f32x4*>(part + (s * heads + at) * d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
+    total += f * x.y;
+    if (x.x != -INFINITY) o += f * y;
   }
-  total = wave_sum(total);
-  __syncthreads();
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = w; s < used; s += 4) {
-    const float f = weight[s];
-    if (f == 0.f && p[s * step + d] == -INFINITY) continue;
+  for (int x = lanes; x < 64; x *= 2) {
+    total += __shfl_xor(total, x, 64);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q * 64 + lane < d) o[q] += f * p[s * step + q * 64 + lane];
+    for (int r = 0; r < 4; ++r) o[r] += __shfl_xor(o[r], x, 64);
   }
+  if constexpr (WAVES == 4) {
+    if (lane < lanes) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) sum[w][q * 64 + lane] = o[q];
-  __syncthreads();
-  if (tid < d) {
-    const float x = ((sum[0][tid] + sum[1][tid]) + sum[2][tid]) + sum[3][tid];
-    st_from_f32<T>((T*)a.out + t * a.o_st + hq * a.o_sh + tid, top == -INFINITY ? 0.f : x / total);
+      for (int r = 0; r < 4; ++r)
+        if (col + r < d) sums[w][col + r] = o[r];
+    }
+    __shared__ float totals[4];
+    if (lane == 0) totals[w] = total;
+    __syncthreads();
+    if (w != 0) return;
+    total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    if (col < d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = (sums[0][col + r] + sums[1][col + r]) + (sums[2][col + r] + sums[3][col + r]);
   }
-  if (a.lse && tid == 0) a.lse[t * a.q_heads + hq] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
+  const float inv = top == -INFINITY ? 0.f : 1.f / total;
+  if (lane < lanes && col < d) {
+    const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    st4_from_f32<T>((T*)a.out + t * a.o_st + hq * a.o_sh + col, y);
+  }
+  if (a.lse && lane == 0) a.lse[at] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
 }
 
 // How a call is cut: rows of a tile, tiles of a sequence, ranges of the keys.
@@ -556,10 +595,10 @@ Cut cut_of(const s2t_paged_args* a) {
   c.mt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
   c.tiles = (int)((rows + 16 * c.mt - 1) / (16 * c.mt));
   const int64_t units = (int64_t)c.tiles * a->kv_heads * a->B, keys = (int64_t)a->table_pages * a->page_size;
-  int64_t s = (2048 + units - 1) / units;
-  const int64_t can = (keys + MIN_CHUNK - 1) / MIN_CHUNK;
-  if (s > can) s = can;
+  int64_t s = (c.mt * a->dk > 128 ? 256 : 512) / units;
+  if (s > keys / MIN_CHUNK) s = keys / MIN_CHUNK;
   if (s > 256) s = 256;
+  if (s < 1) s = 1;
   c.splits = (int)s;
   return c;
 }
@@ -589,9 +628,14 @@ void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
   } else {
     launch_attention<T, 256, 1>(a, c, st);
   }
-  if (c.splits > 1)
-    hipLaunchKernelGGL(paged_combine_kernel<T>, dim3((unsigned)(a->max_new * a->q_heads), (unsigned)a->B), dim3(256), 0, st, *a,
-                       __builtin_ctz((unsigned)a->page_size), 16 * c.mt, c.splits, (const float*)a->ws);
+  if (c.splits > 1) {
+    const int rows = a->max_new * a->q_heads, shift = __builtin_ctz((unsigned)a->page_size);
+    const int lanes = a->dk <= 16 ? 4 : a->dk <= 32 ? 8 : a->dk <= 64 ? 16 : a->dk <= 128 ? 32 : 64;
+    if (c.splits <= 8)
+      hipLaunchKernelGGL((paged_combine_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4), (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, lanes, (const float*)a->ws);
+    else
+      hipLaunchKernelGGL((paged_combine_kernel<T, 4>), dim3((unsigned)rows, (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, lanes, (const float*)a->ws);
+  }
 }
 
 int paged_args_bad(const s2t_paged_args* a) {
@@ -645,7 +689,7 @@ extern "C" int s2t_paged_attention(const s2t_paged_args* a, void* stream) {
   const Cut c = cut_of(a);
   const int64_t blocks = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8 * c.tiles * c.splits;
   // launch bounds, and 32-bit offsets of the 16 rows of a half tile
-  if (blocks > 0x7fffffff || (int64_t)a->max_new * a->q_heads > 0x7fffffff || a->p_sr < 0 || a->p_sr > (1 << 24)) return S2T_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffff || (int64_t)a->max_new * a->q_heads > 0x7ffffff0 || a->p_sr < 0 || a->p_sr > (1 << 24)) return S2T_ERR_UNSUPPORTED;
   if (c.splits > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < s2t_paged_attention_ws_bytes(a))) return S2T_ERR_ARG;
   if (a->dtype == S2T_F32) launch_attention<float>(a, c, (hipStream_t)stream);
   else launch_attention<bf16_t>(a, c, (hipStream_t)stream);
