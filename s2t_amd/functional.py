@@ -2328,28 +2328,32 @@ class TokenScores(NamedTuple):
 NO_IGNORE = -(1 << 63)
 
 
+def _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, want_lse):
+    """-> logprob, entropy, top_logprob, top_index, lse of rows of logits [rows, V]; None for what is not asked for."""
+    rows, dev = logits.shape[0], logits.device
+    f32 = torch.float32
+    logprob = torch.empty(rows, dtype=f32, device=dev) if tokens is not None else None
+    lse = torch.empty(rows, dtype=f32, device=dev) if want_lse else None
+    entropy = torch.empty(rows, dtype=f32, device=dev) if want_entropy else None
+    top_lp = torch.empty(rows, top, dtype=f32, device=dev) if top else None
+    top_idx = torch.empty(rows, top, dtype=torch.int64, device=dev) if top else None
+    K.token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_lp, top_idx)
+    return logprob, entropy, top_lp, top_idx, lse
+
+
 class TokenLogprobsFn(torch.autograd.Function):
     """Log probabilities of ``tokens`` under rows of logits, entropies and the best alternatives, and their gradient
     (sequence_scorer.py:75-110); the row statistics are saved, the probabilities are formed again in the backward pass."""
 
     @staticmethod
     def forward(ctx, logits, tokens, ignore_index, inv_temp, top, want_entropy):
-        rows, V = logits.shape
-        f32 = dict(dtype=torch.float32, device=logits.device)
-        logprob = torch.empty(rows, **f32) if tokens is not None else None
-        train = ctx.needs_input_grad[0]
-        lse = torch.empty(rows, **f32) if train else None
-        entropy = torch.empty(rows, **f32) if want_entropy else None
-        top_lp = torch.empty(rows, top, **f32) if top else None
-        top_idx = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
-        K.token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_lp, top_idx)
-        if train:
-            ctx.save_for_backward(logits, tokens, lse, entropy, top_idx)
-            ctx.args = (ignore_index, inv_temp, top)
-            ctx.set_materialize_grads(False)
-            if top_idx is not None:
-                ctx.mark_non_differentiable(top_idx)
-        return logprob, entropy, top_lp, top_idx
+        *out, lse = _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, True)
+        ctx.save_for_backward(logits, tokens, lse, out[1], out[3])
+        ctx.args = (ignore_index, inv_temp, top)
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(out[3])
+        return tuple(out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -2370,28 +2374,35 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
     rows padded to a multiple of 8, as the output projection returns them, is read in place), ``tokens`` [...] int64.
     Rows whose token is ``ignore_index`` score 0 (top_index -1), are not read and get no gradient; a token outside the vocabulary scores
     NaN.  All results are fp32, differentiable with respect to the logits (once).  -> ``TokenScores``"""
-    if logits.dim() < 1 or logits.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("token_logprobs: logits [..., V] in float32 or bfloat16 expected, got %s %s" % (tuple(logits.shape), logits.dtype))
-    V, lead = logits.shape[-1], logits.shape[:-1]
+    shape = logits.shape
+    if not shape or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("token_logprobs: logits [..., V] in float32 or bfloat16 expected, got %s %s" % (tuple(shape), logits.dtype))
+    V, lead = shape[-1], shape[:-1]
     if V < 1 or not 0 <= top <= min(V, 64):
         raise ValueError("token_logprobs: top = %s of a vocabulary of %d (at most 64)" % (top, V))
-    if not temperature > 0 or temperature == math.inf:
+    if not 0 < temperature < math.inf:
         raise ValueError("token_logprobs: temperature must be positive, got %s" % temperature)
-    if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != lead or tokens.device != logits.device):
+    if tokens is not None and (tokens.dtype is not torch.int64 or tokens.shape != lead or tokens.device != logits.device):
         raise ValueError("token_logprobs: tokens must be int64 of shape %s on %s, got %s %s on %s" % (
             tuple(lead), logits.device, tokens.dtype, tuple(tokens.shape), tokens.device))
     if tokens is None and not top and not entropy:
         raise ValueError("token_logprobs: nothing asked for (tokens, top or entropy)")
-    require_cuda(logits, tokens)
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.shape[0] and (x.stride(1) != 1 and V > 1 or x.stride(0) < V):
+    require_cuda(logits)
+    flat = len(shape) == 2
+    x = logits if flat else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1 or x.stride(0) < V:
         x = x.contiguous()
-    y = None if tokens is None else tokens.reshape(-1).contiguous()
-    r = TokenLogprobsFn.apply(x, y, NO_IGNORE if ignore_index is None else int(ignore_index), 1.0 / temperature, int(top), bool(entropy))
-    if logits.dim() == 2:
-        return TokenScores(*r)
-    shape = lambda t: None if t is None else t.view(lead + t.shape[1:])  # noqa: E731
-    return TokenScores(*(shape(t) for t in r))
+    y = tokens
+    if y is not None and not (flat and y.is_contiguous()):
+        y = y.reshape(-1).contiguous()
+    args = (x, y, NO_IGNORE if ignore_index is None else int(ignore_index), 1.0 / temperature, int(top), bool(entropy))
+    if torch.is_grad_enabled() and x.requires_grad:
+        r = TokenLogprobsFn.apply(*args)
+    else:
+        r = _score_rows(*args, False)[:4]
+    if not flat:
+        r = [None if t is None else t.view(lead + t.shape[1:]) for t in r]
+    return TokenScores(*r)
 
 
 def _side_stream(device):

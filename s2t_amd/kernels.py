@@ -1005,53 +1005,54 @@ def wgrad_grouped(problems, n_problems, items, n_items, tiles, n_tiles, ws, any_
 
 
 # ---- paged key/value cache, token scores ---------------------------------------------------------------------------------------
+_ENTRIES = {}
+
+
 def _call_on(device, name, *args):
-    """``_call`` on the device that the tensors live on and its current stream, whichever device is the current one."""
-    fn = getattr(L.lib(), name)
-    if device.index == torch.cuda.current_device():
-        L.check(fn(*args, L.stream_ptr()), name)
+    """``_call`` on the device (its index) that the tensors live on and its current stream, whichever device is the current one."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(L.lib(), name)
+    if device == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            L.check(fn(*args, L.stream_ptr()), name)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        L.check(status, name)
 
 
-def paged_args(k_pages, v_pages, page_table, lens, cu, N, max_new, q_heads):
-    """The part of s2t_paged_args (include/s2t_hip.h) that append and attention share; shapes and types are the caller's to check."""
-    a = L.PagedArgs()
-    a.dtype = L.S2T_F32 if k_pages.dtype == torch.float32 else L.S2T_BF16
-    P, H, S, d = k_pages.shape
-    a.B, a.N, a.max_new = lens.shape[0], N, max_new
-    a.q_heads, a.kv_heads, a.dk = q_heads, H, d
-    a.num_pages, a.page_size, a.table_pages = P, S, page_table.shape[1]
-    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    a.p_sp, a.p_sh, a.p_sr, _ = k_pages.stride()
-    a.page_table, a.table_stride = page_table.data_ptr(), page_table.stride(0)
-    a.lens, a.cu = lens.data_ptr(), cu.data_ptr()
-    return a
+def paged_kv_append(device, *fields):
+    """s2t_paged_kv_append; ``fields``: those of s2t_paged_args (include/s2t_hip.h) in order, the attention's left out."""
+    _call_on(device, "s2t_paged_kv_append", L.PAGED_ARGS.pack(*fields, *_NO_ATTENTION))
 
 
-def paged_kv_append(a, device):
-    _call_on(device, "s2t_paged_kv_append", C.byref(a))
+_NO_ATTENTION = (0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0)
+_NO_APPEND = (0, 0, 0, 0, 0, 0, 0, 0, 0)
+PAGED_ONE_RANGE = 1023  # up to so many places of a sequence the attention needs no workspace (csrc/paged.hip, cut_of)
 
 
-def paged_attention(a, device):
-    """Runs s2t_paged_attention; its workspace comes from the allocator (a captured graph keeps its own)."""
-    n = L.lib().s2t_paged_attention_ws_bytes(C.byref(a))
-    ws = None
-    if n > 0:
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
-        a.ws, a.ws_bytes = ws.data_ptr(), n
-    _call_on(device, "s2t_paged_attention", C.byref(a))
+def paged_attention(device, cache, q, out_to_scale):
+    """s2t_paged_attention; the workspace comes from the allocator (a captured graph keeps its own).  ``cache``: the fields up to cu,
+    ``q``: its address and strides, ``out_to_scale``: out .. scale."""
+    head = cache + (0, 0, 0, 0, 0, 0) + q + _NO_APPEND + out_to_scale
+    args = L.PAGED_ARGS.pack(*head, 0, 0)
+    if cache[8] * cache[9] > PAGED_ONE_RANGE:
+        n = L.lib().s2t_paged_attention_ws_bytes(args)
+        if n > 0:
+            ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", device))
+            args = L.PAGED_ARGS.pack(*head, ws.data_ptr(), n)
+    _call_on(device, "s2t_paged_attention", args)
 
 
 def token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index):
     rows, V = logits.shape
-    _call_on(logits.device, "s2t_token_logprobs_fwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0), rows, V, _ptr(tokens),
+    _call_on(logits.get_device(), "s2t_token_logprobs_fwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, _ptr(tokens),
              ignore_index, inv_temp, top, _ptr(logprob), _ptr(lse), _ptr(entropy), _ptr(top_logprob), _ptr(top_index))
 
 
 def token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits):
     rows, V = logits.shape
-    _call_on(logits.device, "s2t_token_logprobs_bwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0), rows, V, _ptr(tokens),
+    _call_on(logits.get_device(), "s2t_token_logprobs_bwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, _ptr(tokens),
              ignore_index, inv_temp, top, _ptr(lse), _ptr(entropy), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(top_index),
              dlogits.data_ptr(), dlogits.stride(0))

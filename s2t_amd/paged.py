@@ -23,6 +23,10 @@ from . import _lib as L
 from . import kernels as K
 
 _TYPES = (torch.float32, torch.bfloat16)
+_I32 = torch.int32
+
+
+_NONE3 = (0, 0, 0)
 
 
 def _refuse(what):
@@ -30,6 +34,7 @@ def _refuse(what):
 
 
 def _check_cache(k_pages, v_pages, page_table, lens, cu, max_new):
+    """Raises for what is wrong with a cache."""
     if k_pages.dim() != 4 or k_pages.dtype not in _TYPES or v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape:
         _refuse("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim] of one type (float32 or bfloat16), got %s %s and %s %s" % (
             tuple(k_pages.shape), k_pages.dtype, tuple(v_pages.shape), v_pages.dtype))
@@ -45,30 +50,55 @@ def _check_cache(k_pages, v_pages, page_table, lens, cu, max_new):
         _refuse("lens must be int32 [%d], contiguous" % B)
     if cu.dtype != torch.int32 or tuple(cu.shape) != (B + 1,) or not cu.is_contiguous():
         _refuse("cu must be int32 [%d], contiguous" % (B + 1))
-    if not 1 <= B <= 65535 or max_new < 0:
-        _refuse("1 to 65535 sequences and max_new >= 0 expected, got %d and %s" % (B, max_new))
+    if not 1 <= B <= 65535 or not 0 <= max_new < 1 << 31:
+        _refuse("1 to 65535 sequences and 0 <= max_new < 2^31 expected, got %d and %s" % (B, max_new))
 
 
-def _check_rows(name, t, heads, like, n=None):
-    if t.dim() != 3 or t.dtype != like.dtype or (heads is not None and t.shape[1] != heads) or t.shape[2] != like.shape[3] or t.stride(2) != 1 \
-            or (n is not None and t.shape[0] != n):
+def _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, q_heads):
+    """-> the fields of s2t_paged_args up to cu, head_dim, kv_heads.  One look at everything; what fails it is named by _check_cache."""
+    kind, shape, stride, of_table = k_pages.dtype, k_pages.shape, k_pages.stride(), page_table.shape
+    if len(shape) == 4 and len(of_table) == 2:
+        P, H, S, d = shape
+        B, n = of_table
+        if (kind in _TYPES and v_pages.dtype is kind and v_pages.shape == shape and v_pages.stride() == stride and stride[3] == 1
+                and P > 0 and H > 0 and S > 0 and not S & (S - 1) and not d % 16 and 16 <= d <= 256 and n > 0 and 0 < B < 65536
+                and page_table.dtype is lens.dtype is cu.dtype is _I32 and (page_table.stride(1) == 1 or n == 1)
+                and lens.shape == (B,) and cu.shape == (B + 1,) and lens.is_contiguous() and cu.is_contiguous() and 0 <= max_new < 1 << 31
+                and N < 1 << 31):
+            if q_heads < 1 or q_heads % H:
+                _refuse("%d query heads over %d key/value heads" % (q_heads, H))
+            return (L.S2T_F32 if kind is torch.float32 else L.S2T_BF16, B, N, max_new, q_heads, H, d, P, S, n, k_pages.data_ptr(),
+                    v_pages.data_ptr(), stride[0], stride[1], stride[2], page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), cu.data_ptr())
+    _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
+    _refuse("%d rows" % N)
+
+
+def _rows(name, t, heads, like, n=None):
+    """-> address and strides of [n, heads, head_dim]."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype is not like.dtype or shape[2] != like.shape[3] or stride[2] != 1 or (heads is not None and shape[1] != heads) \
+            or (n is not None and shape[0] != n):
         _refuse("%s must be [%s, %s, %d] %s with a contiguous last dimension, got %s %s" % (
-            name, "rows" if n is None else n, "heads" if heads is None else heads, like.shape[3], like.dtype, tuple(t.shape), t.dtype))
+            name, "rows" if n is None else n, "heads" if heads is None else heads, like.shape[-1], like.dtype, tuple(shape), t.dtype))
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _check_index(name, t, n):
-    if t.dtype != torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+def _index(name, t, n):
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         _refuse("%s must be int32 [%d], contiguous" % (name, n))
+    return t.data_ptr()
 
 
-def _one_device(*tensors):
-    L.require_cuda(*tensors)
-    dev = tensors[0].device
+def _device(*tensors):
+    """-> index of the one device that all of them (None aside) live on."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            _refuse("tensors on %s and %s" % (dev, t.device))
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the paged cache is inference only: wrap the decoder in torch.no_grad()")
+        if t is not None and t.get_device() != dev or dev < 0:
+            L.require_cuda(*tensors)
+            _refuse("tensors on several devices: %s" % ", ".join(str(t.device) for t in tensors if t is not None))
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors if t is not None]):
+        raise RuntimeError("the paged cache is inference only: wrap the decoder in torch.no_grad()")
+    return dev
 
 
 def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=None, rotary=None, positions=None, rows=None, q_out=None):
@@ -80,45 +110,31 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
     into ``q_out`` (default: a new tensor; ``q`` itself: in place) and returned.
     ``rows`` (int32 [N], instead of q): new token t takes row ``rows[t]`` of k and v — the accepted drafts of a verified tree, whose
     projections the caller has kept; a row outside k is not stored."""
-    _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
-    _check_rows("k", k, k_pages.shape[1], k_pages)
-    _check_rows("v", v, k_pages.shape[1], k_pages, k.shape[0])
-    N = k.shape[0] if rows is None else rows.shape[0]
-    if rows is not None:
-        if q is not None:
-            _refuse("q cannot be turned together with a selection of rows")
-        _check_index("rows", rows, N)
-    if positions is not None:
-        _check_index("positions", positions, N)
-    if max_new >= 1 << 31 or N >= 1 << 31:
-        _refuse("%d new tokens" % max(N, max_new))
-    a = K.paged_args(k_pages, v_pages, page_table, lens, cu, N, max_new, k_pages.shape[1] if q is None else q.shape[1])
-    a.k, a.k_st, a.k_sh = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_st, a.v_sh = v.data_ptr(), v.stride(0), v.stride(1)
-    if rotary is not None:
-        if rotary.dtype != torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.shape[0] < 1 \
-                or rotary.shape[1] % 16 or not 16 <= rotary.shape[1] <= k_pages.shape[3]:
-            _refuse("rotary must be float32 [positions, rot_dim], contiguous, rot_dim a multiple of 16 up to head_dim, got %s %s" % (
-                tuple(rotary.shape), rotary.dtype))
-        a.rotary, (a.rotary_positions, a.rot_dim) = rotary.data_ptr(), rotary.shape
+    N = k.shape[0] if rows is None else rows.shape[0] if rows.dim() else -1
+    cache = _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, k_pages.shape[1] if q is None else q.shape[1] if q.dim() > 1 else 0)
+    kf = _rows("k", k, cache[5], k_pages)
+    vf = _rows("v", v, cache[5], k_pages, k.shape[0])
+    qf = of = _NONE3
     if q is not None:
-        _check_rows("q", q, None, k_pages, N)
-        if q.shape[1] < 1 or q.shape[1] % k_pages.shape[1]:
-            _refuse("%d query heads over %d key/value heads" % (q.shape[1], k_pages.shape[1]))
+        if rows is not None:
+            _refuse("q cannot be turned together with a selection of rows")
+        qf = _rows("q", q, None, k_pages, N)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        else:
-            _check_rows("q_out", q_out, q.shape[1], k_pages, N)
-        a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-        a.q_out, a.qo_st, a.qo_sh = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+            q_out = torch.empty_like(q)
+        of = _rows("q_out", q_out, cache[4], k_pages, N)
     elif q_out is not None:
         _refuse("q_out without q")
-    _one_device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out)
-    if positions is not None:
-        a.positions = positions.data_ptr()
-    if rows is not None:
-        a.rows, a.src_rows = rows.data_ptr(), k.shape[0]
-    K.paged_kv_append(a, k_pages.device)
+    turn = _NONE3
+    if rotary is not None:
+        if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.shape[0] < 1 \
+                or rotary.shape[1] % 16 or not 16 <= rotary.shape[1] <= cache[6]:
+            _refuse("rotary must be float32 [positions, rot_dim], contiguous, rot_dim a multiple of 16 up to head_dim, got %s %s" % (
+                tuple(rotary.shape), rotary.dtype))
+        turn = (rotary.data_ptr(),) + tuple(rotary.shape)
+    at = _index("positions", positions, N) if positions is not None else 0
+    pick = _index("rows", rows, N) if rows is not None else 0
+    dev = _device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out)
+    K.paged_kv_append(dev, *cache, *kf, *vf, *qf, *of, *turn, at, pick, k.shape[0])
     return q_out
 
 
@@ -130,27 +146,21 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
     ``[N, words]``) new token j where bit ``j % 64`` of word ``j // 64`` of its row is set — its ancestors and itself, any other set will do.
     A row that sees nothing comes out 0 with lse -inf; what a row does not see never touches it, infinities and NaN included.
     Inference only.  -> out [N, q_heads, head_dim] (``out`` if given), with ``return_lse`` also the fp32 logsumexp [N, q_heads]."""
-    _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
-    _check_rows("q", q, None, k_pages)
-    N, Hq, d = q.shape
-    if Hq < 1 or Hq % k_pages.shape[1] or Hq > 65535 or max_new >= 1 << 31 or N >= 1 << 31:
-        _refuse("%d query heads over %d key/value heads, %d new tokens" % (Hq, k_pages.shape[1], N))
-    a = K.paged_args(k_pages, v_pages, page_table, lens, cu, N, max_new, Hq)
+    N, Hq, d = q.shape if q.dim() == 3 else (0, 0, 0)
+    cache = _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, Hq)
+    qf = _rows("q", q, None, k_pages)
+    bits = _NONE3
     if tree is not None:
-        if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
+        if tree.dtype is not torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
             _refuse("tree must be int64 [%d, words] with contiguous rows, got %s %s" % (N, tuple(tree.shape), tree.dtype))
-        a.tree, a.tree_stride, a.tree_words = tree.data_ptr(), tree.stride(0), tree.shape[1]
+        bits = (tree.data_ptr(), tree.stride(0), tree.shape[1])
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_rows("out", out, Hq, k_pages, N)
-    _one_device(k_pages, v_pages, page_table, lens, cu, q, tree, out)
-    a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-    a.out, a.o_st, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
-    a.scale = d ** -0.5 if scale is None else float(scale)
-    lse = None
+        out = torch.empty_like(q)
+    of = _rows("out", out, Hq, k_pages, N)
+    dev = _device(k_pages, v_pages, page_table, lens, cu, q, tree, out)
+    lse, to_lse = None, 0
     if return_lse:
         lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device)
-        a.lse = lse.data_ptr()
-    K.paged_attention(a, q.device)
+        to_lse = lse.data_ptr()
+    K.paged_attention(dev, cache, qf, of + (to_lse,) + bits + (d ** -0.5 if scale is None else float(scale),))
     return (out, lse) if return_lse else out

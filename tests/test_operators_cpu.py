@@ -24,7 +24,23 @@ def _struct_fields(name):
 
 
 def test_paged_struct_matches_header_field_order():
-    assert _struct_fields("s2t_paged_args") == [f[0] for f in L.PagedArgs._fields_]
+    """Names in order, and the packed record as the compiler lays the struct out (8-byte fields on 8 bytes)."""
+    assert _struct_fields("s2t_paged_args") == L.PAGED_FIELDS
+    codes = L.PAGED_ARGS.format.replace("@", "").replace("10i", "i" * 10).replace(" ", "")
+    types = {"P": C.c_void_p, "q": C.c_int64, "i": C.c_int32, "f": C.c_float}
+    mirror = type("Mirror", (C.Structure,), {"_fields_": [(n, types[c]) for n, c in zip(L.PAGED_FIELDS, codes)]})
+    assert len(codes) == len(L.PAGED_FIELDS) and C.sizeof(mirror) == L.PAGED_ARGS.size
+    m = mirror.from_buffer_copy(L.PAGED_ARGS.pack(*range(1, 1 + len(codes))))
+    assert [int(getattr(m, n) or 0) for n in L.PAGED_FIELDS] == list(range(1, 1 + len(codes)))
+    import re
+    src = re.sub(r"/\*.*?\*/", "", open(L.HEADER_PATH).read(), flags=re.S)
+    body = src[src.index("typedef struct s2t_paged_args {") + len("typedef struct s2t_paged_args {"):src.index("} s2t_paged_args;")]
+    got = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        first, *more = decl.split(",")
+        kind = "P" if "*" in first else {"int32_t": "i", "int64_t": "q", "float": "f"}[first.split()[0]]
+        got += [kind] * (1 + len(more))
+    assert "".join(got) == codes
 
 
 def _good(dtype=torch.float32, B=3, N=5, H=2, Hq=4, d=32, S=16, P=7):
@@ -120,29 +136,31 @@ def test_bad_scores_are_refused():
 def test_the_c_entries_refuse_before_they_launch():
     lib = L.lib()
     assert lib.s2t_paged_kv_append(None, None) == -1 and lib.s2t_paged_attention(None, None) == -1
-    a = L.PagedArgs()
-    assert lib.s2t_paged_attention(C.byref(a), None) == -1
+    assert lib.s2t_paged_attention(bytes(L.PAGED_ARGS.size), None) == -1
     buf = torch.zeros(64, dtype=torch.float64)
     p = buf.data_ptr()
     p += -p % 16
 
     def args(**change):
-        a = L.PagedArgs(dtype=0, B=1, N=0, max_new=1, q_heads=2, kv_heads=1, dk=32, num_pages=1, page_size=16, table_pages=1, k_pages=p, v_pages=p,
+        a = dict(dtype=0, B=1, N=0, max_new=1, q_heads=2, kv_heads=1, dk=32, num_pages=1, page_size=16, table_pages=1, k_pages=p, v_pages=p,
                         p_sp=512, p_sh=512, p_sr=32, page_table=p, table_stride=1, lens=p, cu=p, k=p, k_st=32, k_sh=32, v=p, v_st=32, v_sh=32, q=p,
                         q_st=64, q_sh=32, q_out=p, qo_st=64, qo_sh=32, out=p, o_st=64, o_sh=32, scale=1.0)
-        for k, v in change.items():
-            setattr(a, k, v)
-        return a
+        a.update(change)
+        return L.PAGED_ARGS.pack(*(a.get(n) or (0.0 if n == "scale" else 0) for n in L.PAGED_FIELDS))
 
     for entry in (lib.s2t_paged_kv_append, lib.s2t_paged_attention):
-        assert entry(C.byref(args()), None) == 0  # no rows: nothing is launched
+        assert entry(args(), None) == 0  # no rows: nothing is launched
         for status, change in ((-2, dict(dtype=2)), (-1, dict(B=0)), (-1, dict(B=65536)), (-1, dict(page_size=24)), (-1, dict(q_heads=3, kv_heads=2)),
                                (-4, dict(dk=24)), (-4, dict(dk=272)), (-1, dict(num_pages=0)), (-1, dict(lens=None)), (-3, dict(k_pages=p + 4)),
                                (-3, dict(p_sr=33)), (-3, dict(q_st=66)), (-4, dict(table_pages=1 << 27))):
-            assert entry(C.byref(args(**change)), None) == status, change
-    assert lib.s2t_paged_kv_append(C.byref(args(rows=p)), None) == -1            # with q
-    assert lib.s2t_paged_kv_append(C.byref(args(rotary=p, rot_dim=48, rotary_positions=1)), None) == -1
-    assert lib.s2t_paged_attention(C.byref(args(tree=p, tree_words=0)), None) == -1
+            assert entry(args(**change), None) == status, change
+    from s2t_amd import kernels as K
+    ws = lambda **change: lib.s2t_paged_attention_ws_bytes(args(N=5, max_new=5, **change))  # noqa: E731
+    assert ws(table_pages=K.PAGED_ONE_RANGE // 16) == ws(page_size=1, table_pages=K.PAGED_ONE_RANGE) == 0 < ws(table_pages=1 << 16)
+    assert lib.s2t_paged_attention(args(N=5, max_new=5, table_pages=1 << 16), None) == -1   # no workspace
+    assert lib.s2t_paged_kv_append(args(rows=p), None) == -1            # with q
+    assert lib.s2t_paged_kv_append(args(rotary=p, rot_dim=48, rotary_positions=1), None) == -1
+    assert lib.s2t_paged_attention(args(tree=p, tree_words=0), None) == -1
     f, b = lib.s2t_token_logprobs_fwd, lib.s2t_token_logprobs_bwd
     assert f(0, p, 8, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == 0
     assert f(0, p, 7, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == -1       # rows overlap
