@@ -1,5 +1,6 @@
 // Paged key/value cache of an incremental decoder: append (with rotary positions on the way) and attention of several new tokens of a
 // sequence over it, chain or tree of drafts.  Layout, bounds and semantics: include/s2t_hip.h, s2t_paged_args.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -31,58 +32,96 @@ __device__ __forceinline__ Span span_of(const s2t_paged_args& a, int b) {
 }
 
 // ---- append -----------------------------------------------------------------------------------------------------------------
-// One workgroup per new token; a thread moves 16 bytes (two times 16 where elements turn in pairs).
+// A wave takes TOKENS new tokens of a sequence; its lanes go over the units of a token (16 bytes that pass, or two times 16 that turn
+// together: first all of k, then v, then q), each for all of its tokens at once, so that TOKENS loads are on their way before the first
+// store and what a unit is has to be worked out once.  Where the tokens go comes by scalar loads.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args a, int shift) {
-  const int b = blockIdx.y, i = blockIdx.x;
-  const Span s = span_of(a, b);
-  if (i >= s.n) return;
-  const int t = s.row0 + i, place = s.len - s.n + i;
-  const int64_t to = pages_of(a, shift, b).at(place);
-  constexpr int E = 16 / (int)sizeof(T);
-  const int rot = a.rotary ? a.rot_dim : 0, half = rot / 2;
-  const int pos = a.positions ? a.positions[t] : place;
-  const bool known = (uint32_t)pos < (uint32_t)a.rotary_positions;
-  const float* cs = a.rotary + (int64_t)(known ? pos : 0) * rot;
-  const int row = a.rows ? a.rows[t] : t;
-  const bool stored = to >= 0 && (!a.rows || (uint32_t)row < (uint32_t)a.src_rows);
-  // units of a head: `half / E` pairs of vectors that turn together, then the vectors that pass
-  const int pairs = half / E, units = pairs + (a.dk - rot) / E;
-  auto turn = [&](const T* src, T* dst, int u) {
-    if (u >= pairs) {
-      const int c = rot + (u - pairs) * E;
-      *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-      return;
-    }
-    float x[E], y[E];
+struct Turned {
+  static constexpr int E = 16 / (int)sizeof(T);
+  // (x, y) -> (x cos - y sin, y cos + x sin), cs: cosines of this unit, sines `half` floats behind; rounded once
+  static __device__ __forceinline__ void turn(uint4& xv, uint4& yv, const float* cs, int half, bool known) {
+    uint32_t* xw = reinterpret_cast<uint32_t*>(&xv);
+    uint32_t* yw = reinterpret_cast<uint32_t*>(&yv);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = ld_as_f32<T>(src + u * E + e);
-      y[e] = ld_as_f32<T>(src + half + u * E + e);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float c = known ? cs[u * E + e] : __builtin_nanf(""), sn = known ? cs[half + u * E + e] : __builtin_nanf("");
-      st_from_f32<T>(dst + u * E + e, x[e] * c - y[e] * sn);
-      st_from_f32<T>(dst + half + u * E + e, y[e] * c + x[e] * sn);
-    }
-  };
-  if (stored) {
-    for (int w = threadIdx.x; w < a.kv_heads * units; w += 256) {
-      const int h = w / units, u = w % units;
-      turn((const T*)a.k + row * a.k_st + h * a.k_sh, (T*)a.k_pages + to + h * a.p_sh, u);
-    }
-    const int vecs = a.dk / E;
-    for (int w = threadIdx.x; w < a.kv_heads * vecs; w += 256) {
-      const int h = w / vecs, c = (w % vecs) * E;
-      *reinterpret_cast<uint4*>((T*)a.v_pages + to + h * a.p_sh + c) =
-          *reinterpret_cast<const uint4*>((const T*)a.v + row * a.v_st + h * a.v_sh + c);
+    for (int q = 0; q < E / 4; ++q) {
+      float4 c = reinterpret_cast<const float4*>(cs)[q], s = reinterpret_cast<const float4*>(cs + half)[q];
+      if (!known) c.x = c.y = c.z = c.w = __builtin_nanf("");  // NaN both ways: x nan - y s, y nan + x s
+      if constexpr (sizeof(T) == 2) {
+        const float x0 = __uint_as_float(xw[2 * q] << 16), x1 = __uint_as_float(xw[2 * q] & 0xffff0000u);
+        const float x2 = __uint_as_float(xw[2 * q + 1] << 16), x3 = __uint_as_float(xw[2 * q + 1] & 0xffff0000u);
+        const float y0 = __uint_as_float(yw[2 * q] << 16), y1 = __uint_as_float(yw[2 * q] & 0xffff0000u);
+        const float y2 = __uint_as_float(yw[2 * q + 1] << 16), y3 = __uint_as_float(yw[2 * q + 1] & 0xffff0000u);
+        xw[2 * q] = bf16pack(x0 * c.x - y0 * s.x, x1 * c.y - y1 * s.y);
+        xw[2 * q + 1] = bf16pack(x2 * c.z - y2 * s.z, x3 * c.w - y3 * s.w);
+        yw[2 * q] = bf16pack(y0 * c.x + x0 * s.x, y1 * c.y + x1 * s.y);
+        yw[2 * q + 1] = bf16pack(y2 * c.z + x2 * s.z, y3 * c.w + x3 * s.w);
+      } else {
+        const float x0 = __uint_as_float(xw[0]), x1 = __uint_as_float(xw[1]), x2 = __uint_as_float(xw[2]), x3 = __uint_as_float(xw[3]);
+        const float y0 = __uint_as_float(yw[0]), y1 = __uint_as_float(yw[1]), y2 = __uint_as_float(yw[2]), y3 = __uint_as_float(yw[3]);
+        xw[0] = __float_as_uint(x0 * c.x - y0 * s.x);
+        xw[1] = __float_as_uint(x1 * c.y - y1 * s.y);
+        xw[2] = __float_as_uint(x2 * c.z - y2 * s.z);
+        xw[3] = __float_as_uint(x3 * c.w - y3 * s.w);
+        yw[0] = __float_as_uint(y0 * c.x + x0 * s.x);
+        yw[1] = __float_as_uint(y1 * c.y + x1 * s.y);
+        yw[2] = __float_as_uint(y2 * c.z + x2 * s.z);
+        yw[3] = __float_as_uint(y3 * c.w + x3 * s.w);
+      }
     }
   }
-  if (a.q) {
-    for (int w = threadIdx.x; w < a.q_heads * units; w += 256) {
-      const int h = w / units, u = w % units;
-      turn((const T*)a.q + t * a.q_st + h * a.q_sh, (T*)a.q_out + t * a.qo_st + h * a.qo_sh, u);
+};
+
+template <typename T, int TOKENS>
+__global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args a, const int shift, const uint32_t by_units, const uint32_t by_vecs) {
+  constexpr int E = Turned<T>::E;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i0 = (blockIdx.x * 4 + wave) * TOKENS;
+  const Span s = span_of(a, b);
+  const int n = min(s.n, a.max_new);
+  if (i0 >= n) return;
+  const Pages pages = pages_of(a, shift, b);
+  const int rot = a.rotary ? a.rot_dim : 0, half = rot / 2;
+  const int pairs = half / E, units = pairs + (a.dk - rot) / E, vecs = a.dk / E;
+  const int nk = a.kv_heads * units, nv = a.kv_heads * vecs, nq = a.q ? a.q_heads * units : 0;
+  int64_t to[TOKENS], from[TOKENS];
+  const float* cs[TOKENS];
+  bool known[TOKENS], stored[TOKENS];
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) {
+    const int i = min(i0 + j, n - 1), t = s.row0 + i, place = s.len - s.n + i;
+    to[j] = pages.at(place);
+    const int row = a.rows ? a.rows[t] : t, pos = a.positions ? a.positions[t] : place;
+    const bool there = !a.rows || (uint32_t)row < (uint32_t)a.src_rows;
+    from[j] = there ? row : 0;
+    known[j] = (uint32_t)pos < (uint32_t)a.rotary_positions;
+    cs[j] = a.rotary + (int64_t)(known[j] ? pos : 0) * rot;
+    stored[j] = i0 + j < n && to[j] >= 0 && there;
+  }
+  for (int u = lane; u < nk + nv + nq; u += 64) {
+    // what this unit is
+    const bool is_v = u >= nk && u < nk + nv, is_q = u >= nk + nv;
+    const int w = is_q ? u - nk - nv : is_v ? u - nk : u, per = is_v ? vecs : units;
+    const int h = per == 1 ? w : (int)__umulhi((uint32_t)w, is_v ? by_vecs : by_units), c = w - h * per;
+    const bool pair = !is_v && c < pairs;
+    const int col = is_v ? c * E : pair ? c * E : rot + (c - pairs) * E;
+    const T* src = (is_v ? (const T*)a.v + h * a.v_sh : is_q ? (const T*)a.q + h * a.q_sh : (const T*)a.k + h * a.k_sh) + col;
+    T* dst = (is_v ? (T*)a.v_pages + h * a.p_sh : is_q ? (T*)a.q_out + h * a.qo_sh : (T*)a.k_pages + h * a.p_sh) + col;
+    const int64_t src_step = is_v ? a.v_st : is_q ? a.q_st : a.k_st;
+    uint4 x[TOKENS], y[TOKENS];
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) {
+      const T* p = src + (is_q ? (int64_t)(s.row0 + min(i0 + j, n - 1)) : from[j]) * src_step;
+      x[j] = *reinterpret_cast<const uint4*>(p);
+      if (pair) y[j] = *reinterpret_cast<const uint4*>(p + half);
+    }
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) {
+      if (pair) Turned<T>::turn(x[j], y[j], cs[j] + c * E, half, known[j]);
+      T* p = dst + (is_q ? (int64_t)(s.row0 + i0 + j) * a.qo_st : to[j]);
+      if (is_q ? i0 + j < n : stored[j]) {
+        *reinterpret_cast<uint4*>(p) = x[j];
+        if (pair) *reinterpret_cast<uint4*>(p + half) = y[j];
+      }
     }
   }
 }
@@ -665,9 +704,15 @@ extern "C" int s2t_paged_kv_append(const s2t_paged_args* a, void* stream) {
     return S2T_ERR_ALIGN;
   if (a->N == 0 || a->max_new == 0 || (a->rows && a->src_rows == 0)) return S2T_OK;  // (an empty tensor has no address)
   if (!a->k || !a->v || (a->q && !a->q_out)) return S2T_ERR_ARG;
-  const dim3 grid((unsigned)a->max_new, (unsigned)a->B);
-  if (a->dtype == S2T_F32) hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a));
-  else hipLaunchKernelGGL(paged_append_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a));
+  const int e = a->dtype == S2T_F32 ? 4 : 8, rot = a->rotary ? a->rot_dim : 0, units = rot / 2 / e + (a->dk - rot) / e, vecs = a->dk / e;
+  if ((int64_t)std::max(a->q_heads, a->kv_heads) * vecs * vecs >= (1ll << 31)) return S2T_ERR_UNSUPPORTED;  // (divisions by reciprocals)
+  const auto by = [](int n) { return n > 1 ? (uint32_t)((1ull << 32) / n + 1) : 0u; };
+  // four tokens to a wave where that still leaves the chip its waves
+  const bool many = (int64_t)a->max_new * a->B >= 16384;
+  const dim3 grid((unsigned)((a->max_new + (many ? 15 : 3)) / (many ? 16 : 4)), (unsigned)a->B);
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs)); };
+  if (a->dtype == S2T_F32) many ? go(paged_append_kernel<float, 4>) : go(paged_append_kernel<float, 1>);
+  else many ? go(paged_append_kernel<bf16_t, 4>) : go(paged_append_kernel<bf16_t, 1>);
   return S2T_LAUNCH_CHECK();
 }
 
