@@ -5,29 +5,57 @@
 namespace {
 
 constexpr int MAX_TOP = 64;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
-// Statistics of a set of z: maximum, s = sum exp(z - m), t = sum exp(z - m) (z - m).  lse = m + log s, entropy = log s - t / s.
+// Statistics of a set of z in powers of two (y = z * log2 e): maximum, s = sum 2^(y - m), t = sum 2^(y - m) (y - m).
+// lse = (m + log2 s) ln 2, entropy = (log2 s - t / s) ln 2.
 struct Stats {
   float m, s, t;
 };
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ Stats merged(Stats a, Stats b) {
   const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
-  const float da = a.m - ref, db = b.m - ref, fa = __expf(da), fb = __expf(db);
+  const float da = a.m - ref, db = b.m - ref, fa = exp2_(da), fb = exp2_(db);
   // a side that fades out contributes no t either: its s * da may be infinite (maximum -inf, or the type's lowest value)
   const float ta = fa == 0.f ? 0.f : fa * (a.t + a.s * da), tb = fb == 0.f ? 0.f : fb * (b.t + b.s * db);
   return {m, a.s * fa + b.s * fb, ta + tb};
 }
+
+// 16 bytes of a row at any element's address (the hardware takes them there)
+struct __attribute__((packed, aligned(2))) Vec {
+  uint32_t w[4];
+};
+template <typename T>
+constexpr int EPV = 16 / (int)sizeof(T);
+template <typename T>
+__device__ __forceinline__ void unpack(const Vec& v, float (&x)[EPV<T>]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * q] = __uint_as_float(v.w[q] << 16);
+      x[2 * q + 1] = __uint_as_float(v.w[q] & 0xffff0000u);
+    } else x[q] = __uint_as_float(v.w[q]);
+  }
+}
+
 struct Best {
   float v;
   int i;
 };
 __device__ __forceinline__ bool before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
 
-template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
-                                                             int64_t ignore, float inv_temp, int top, float* __restrict__ logprob,
-                                                             float* __restrict__ lse_out, float* __restrict__ entropy,
-                                                             float* __restrict__ top_lp, int64_t* __restrict__ top_idx) {
+// One workgroup to a row, one pass: every thread keeps the statistics of its vectors (relative to its own running maximum, moved once
+// for each NB vectors) and, for the alternatives, the maximum of its raw logits.  The top-th largest of the 64 maxima of four threads
+// each bounds the alternatives from below, since as many columns reach it; the threads that do collect their columns that reach it
+// (read once more, from the caches), usually hardly more than `top`, and one wave ranks them by (logit, column).  Rows with more than
+// CAND such columns (ties without end) are ranked one column after the other instead.
+constexpr int CAND = 512;
+template <typename T, int THREADS, bool TOP, bool ENTROPY>
+__global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
+                                                                 int64_t ignore, float inv_temp, int top, float* __restrict__ logprob,
+                                                                 float* __restrict__ lse_out, float* __restrict__ entropy,
+                                                                 float* __restrict__ top_lp, int64_t* __restrict__ top_idx) {
+  constexpr int E = EPV<T>, NB = 5, WAVES = THREADS / 64;  // (five vectors of 256 threads: a row of 10 000 bf16 logits in one go)
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t y = tokens ? tokens[r] : 0;
@@ -35,58 +63,144 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const T* __restrict
     if (tid == 0) {
       if (logprob) logprob[r] = 0.f;
       if (lse_out) lse_out[r] = 0.f;
-      if (entropy) entropy[r] = 0.f;
+      if (ENTROPY) entropy[r] = 0.f;
     }
-    for (int k = tid; k < top; k += 256) {
-      top_lp[r * top + k] = 0.f;
-      top_idx[r * top + k] = -1;
-    }
+    if (TOP)
+      for (int k = tid; k < top; k += THREADS) {
+        top_lp[r * top + k] = 0.f;
+        top_idx[r * top + k] = -1;
+      }
     return;
   }
   const T* row = logits + r * ld;
-  __shared__ Stats part[4];
-  __shared__ Best best[4];
+  const float c2 = inv_temp * LOG2E;
+  const int nvec = V / E, tail = nvec * E + tid;  // thread `tid`: vectors tid, tid + THREADS .., and one of the V % E last columns
   Stats st{-INFINITY, 0.f, 0.f};
-  for (int c = tid; c < V; c += 256) st = merged(st, Stats{ld_as_f32<T>(row + c) * inv_temp, 1.f, 0.f});
+  float most = -INFINITY;
+  auto take = [&](const float* x, int n) __attribute__((always_inline)) {
+    float hi = x[0];
+#pragma unroll
+    for (int e = 1; e < n; ++e) hi = fmaxf(hi, x[e]);
+    if (TOP) most = fmaxf(most, hi);
+    hi *= c2;
+    if (hi > st.m) {
+      const float d = st.m - hi, f = exp2_(d);
+      st.t = ENTROPY && f != 0.f ? f * (st.t + st.s * d) : 0.f;
+      st.s *= f;
+      st.m = hi;
+    }
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+      const float d = fmaf(x[e], c2, -ref), p = exp2_(d);
+      st.s += p;
+      if (ENTROPY) st.t = fmaf(p, fmaxf(d, -1e30f), st.t);  // (a column of -inf: 0 * -1e30)
+    }
+  };
+  for (int v0 = tid; v0 < nvec; v0 += THREADS * NB) {
+    Vec buf[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) buf[u] = *reinterpret_cast<const Vec*>(row + (int64_t)min(v0 + u * THREADS, nvec - 1) * E);
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+      if (v0 + u * THREADS < nvec) {
+        float x[E];
+        unpack<T>(buf[u], x);
+        take(x, E);
+      }
+  }
+  if (tail < V) {
+    const float x = ld_as_f32<T>(row + tail);
+    take(&x, 1);
+  }
+  __shared__ Stats part[WAVES];
+  __shared__ float maxima[TOP ? THREADS : 1];
+  __shared__ Best cand[TOP ? CAND : 1];
+  __shared__ int n_cand;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) st = merged(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)});
   if (lane == 0) part[w] = st;
+  if (TOP) maxima[tid] = most;
+  if (tid == 0) n_cand = 0;
   __syncthreads();
-  st = merged(merged(part[0], part[1]), merged(part[2], part[3]));
-  const float ls = __logf(st.s), lse = st.m + ls;
-  if (tid == 0) {
-    if (lse_out) lse_out[r] = lse;
-    if (entropy) entropy[r] = ls - st.t / st.s;
-    if (logprob && tokens) logprob[r] = (uint64_t)y < (uint64_t)V ? (ld_as_f32<T>(row + y) * inv_temp - st.m) - ls : __builtin_nanf("");
-  }
-  Best last{INFINITY, -1};
-  for (int k = 0; k < top; ++k) {
-    Best b{-INFINITY, 0x7fffffff};
-    for (int c = tid; c < V; c += 256) {
-      const Best x{ld_as_f32<T>(row + c), c};
-      if (before(last, x) && before(x, b)) b = x;
-    }
+  st = part[0];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const Best x{__shfl_xor(b.v, o, 64), __shfl_xor(b.i, o, 64)};
-      if (before(x, b)) b = x;
+  for (int q = 1; q < WAVES; ++q) st = merged(st, part[q]);
+  const float l2 = log2f(st.s);
+  auto score = [&](float x) { return (fmaf(x, c2, -st.m) - l2) * LN2; };
+  if (tid == 0) {
+    if (lse_out) lse_out[r] = (st.m + l2) * LN2;
+    if (ENTROPY) entropy[r] = (l2 - st.t / st.s) * LN2;
+    if (logprob) logprob[r] = (uint64_t)y < (uint64_t)V ? score(ld_as_f32<T>(row + y)) : __builtin_nanf("");
+  }
+  if constexpr (TOP) {
+    // the bound: every wave finds it for itself
+    float bound = maxima[lane];
+#pragma unroll
+    for (int q = 1; q < WAVES; ++q) bound = fmaxf(bound, maxima[q * 64 + lane]);
+    float left = bound;
+    for (int k = 0; k < top; ++k) {
+      bound = wave_max(left);
+      const uint64_t who = __ballot(left == bound);
+      if (lane == (who ? __builtin_ctzll(who) : 0)) left = -INFINITY;
+    }
+    if (most >= bound) {
+      auto offer = [&](float v, int i) {
+        if (v >= bound) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < CAND) cand[at] = Best{v, i};
+        }
+      };
+      for (int v = tid; v < nvec; v += THREADS) {
+        float x[E];
+        unpack<T>(*reinterpret_cast<const Vec*>(row + (int64_t)v * E), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) offer(x[e], v * E + e);
+      }
+      if (tail < V) offer(ld_as_f32<T>(row + tail), tail);
     }
     __syncthreads();
-    if (lane == 0) best[w] = b;
-    __syncthreads();
-    b = best[0];
-    for (int q = 1; q < 4; ++q)
-      if (before(best[q], b)) b = best[q];
-    last = b;
-    if (tid == 0) {
-      top_lp[r * top + k] = (b.v * inv_temp - st.m) - ls;
-      top_idx[r * top + k] = b.i == 0x7fffffff ? -1 : b.i;
+    const int n = n_cand;
+    auto put = [&](int k, Best x) {
+      top_lp[r * top + k] = score(x.v);
+      top_idx[r * top + k] = x.i;
+    };
+    if (n <= CAND) {  // (the order in which they were collected does not matter: no two columns rank alike)
+      for (int j = tid; j < n; j += THREADS) {
+        const Best x = cand[j];
+        int rank = 0;
+        for (int q = 0; q < n; ++q) rank += before(cand[q], x) ? 1 : 0;
+        if (rank < top) put(rank, x);
+      }
+      for (int k = n + tid; k < top; k += THREADS) put(k, Best{__builtin_nanf(""), -1});  // (only NaN left)
+    } else {
+      Best last{INFINITY, -1};
+      for (int k = 0; k < top; ++k) {
+        Best b{-INFINITY, 0x7fffffff};
+        for (int c = tid; c < V; c += THREADS) {
+          const Best x{ld_as_f32<T>(row + c), c};
+          if (before(last, x) && before(x, b)) b = x;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+          const Best x{__shfl_xor(b.v, o, 64), __shfl_xor(b.i, o, 64)};
+          if (before(x, b)) b = x;
+        }
+        __syncthreads();
+        if (lane == 0) cand[w] = b;
+        __syncthreads();
+        b = cand[0];
+        for (int q = 1; q < WAVES; ++q)
+          if (before(cand[q], b)) b = cand[q];
+        last = b;
+        if (tid == 0) put(k, b);
+      }
     }
   }
 }
 
-// d logits of one row: -p (W + g_entropy (log p + H)) / T with W = g_logprob + sum g_top, and the columns of the token and of the
-// alternatives written once more with their own gradient added before the rounding.
+// d logits of one row: -p (W + g_entropy (log p + H)) / T with W = g_logprob + sum g_top; the thread that stored the column of the token or of
+// an alternative stores it once more with its own gradient added before the rounding.
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V,
                                                                  const int64_t* __restrict__ tokens, int64_t ignore, float inv_temp, int top,
@@ -94,35 +208,73 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
                                                                  const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                                                                  const float* __restrict__ g_top, const int64_t* __restrict__ top_idx,
                                                                  T* __restrict__ dlogits, int64_t ldd) {
+  constexpr int E = EPV<T>, NB = 5;
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const T* row = logits + r * ld;
   T* out = dlogits + r * ldd;
+  const int nvec = V / E, tail = nvec * E + tid;
   const int64_t y = tokens ? tokens[r] : -1;
   if (tokens && y == ignore) {
-    for (int c = tid; c < V; c += 256) st_from_f32<T>(out + c, 0.f);
+    for (int v = tid; v < nvec; v += 256) *reinterpret_cast<Vec*>(out + (int64_t)v * E) = Vec{{0, 0, 0, 0}};
+    if (tail < V) st_from_f32<T>(out + tail, 0.f);
     return;
   }
   float gl = g_lp ? g_lp[r] : 0.f;
-  const float ge = g_ent ? g_ent[r] : 0.f, L = lse[r], H = g_ent ? entropy[r] : 0.f;
+  const float ge = g_ent ? g_ent[r] : 0.f, H = g_ent ? entropy[r] : 0.f;
   if (g_lp && (uint64_t)y >= (uint64_t)V) gl = __builtin_nanf("");  // as its score
   float W = gl;
   if (g_top)
     for (int k = 0; k < top; ++k) W += g_top[r * top + k];
-  auto dense = [&](int c) {
-    const float lp = ld_as_f32<T>(row + c) * inv_temp - L, p = __expf(lp);
-    return p == 0.f && W == W ? 0.f : -p * (W + ge * (lp + H));
+  const float c2 = inv_temp * LOG2E, L2 = lse[r] * LOG2E, gw = W + ge * H, gp = ge * LN2;
+  // (a column of -inf: p is 0, and so is its gradient)
+  auto dense = [&](float x) {
+    const float lp = fmaf(x, c2, -L2);
+    return -exp2_(lp) * fmaf(gp, fmaxf(lp, -1e30f), gw);
   };
-  for (int c = tid; c < V; c += 256) st_from_f32<T>(out + c, inv_temp * dense(c));
-  __syncthreads();
-  for (int k = tid; k <= (g_top ? top : 0); k += 256) {
+  for (int v0 = tid; v0 < nvec; v0 += 256 * NB) {
+    Vec buf[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) buf[u] = *reinterpret_cast<const Vec*>(row + (int64_t)min(v0 + u * 256, nvec - 1) * E);
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+      if (v0 + u * 256 < nvec) {
+        float x[E];
+        unpack<T>(buf[u], x);
+        Vec o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (sizeof(T) == 2) o.w[q] = bf16pack(inv_temp * dense(x[2 * q]), inv_temp * dense(x[2 * q + 1]));
+          else o.w[q] = __float_as_uint(inv_temp * dense(x[q]));
+        }
+        *reinterpret_cast<Vec*>(out + (int64_t)(v0 + u * 256) * E) = o;
+      }
+  }
+  if (tail < V) st_from_f32<T>(out + tail, inv_temp * dense(ld_as_f32<T>(row + tail)));
+  for (int k = 0; k <= (g_top ? top : 0); ++k) {
     const int64_t c = k == 0 ? y : top_idx[r * top + k - 1];
     if ((uint64_t)c >= (uint64_t)V || (k == 0 && !g_lp)) continue;
+    if (tid != (c < (int64_t)nvec * E ? (int)(c / E % 256) : (int)(c - (int64_t)nvec * E))) continue;
     float add = c == y ? gl : 0.f;
     if (g_top)
       for (int q = 0; q < top; ++q)
         if (top_idx[r * top + q] == c) add += g_top[r * top + q];
-    st_from_f32<T>(out + c, inv_temp * (dense((int)c) + add));
+    st_from_f32<T>(out + c, inv_temp * (dense(ld_as_f32<T>(row + c)) + add));
+  }
+}
+
+template <typename T, int THREADS>
+void launch_fwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, float* logprob,
+                float* lse, float* entropy, float* top_lp, int64_t* top_idx, hipStream_t s) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, logprob, lse, entropy, top_lp, top_idx);
+  };
+  if (top > 0) {
+    if (entropy) go(token_logprobs_kernel<T, THREADS, true, true>);
+    else go(token_logprobs_kernel<T, THREADS, true, false>);
+  } else {
+    if (entropy) go(token_logprobs_kernel<T, THREADS, false, true>);
+    else go(token_logprobs_kernel<T, THREADS, false, false>);
   }
 }
 
@@ -136,12 +288,9 @@ extern "C" int s2t_token_logprobs_fwd(int dtype, const void* logits, int64_t ld,
   if (dtype != S2T_F32 && dtype != S2T_BF16) return S2T_ERR_DTYPE;
   if (rows == 0) return S2T_OK;  // (an empty tensor has no address)
   if (!logits || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index))) return S2T_ERR_ARG;
-  const dim3 grid((unsigned)rows);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == S2T_F32)
-    hipLaunchKernelGGL(token_logprobs_kernel<float>, grid, dim3(256), 0, s, (const float*)logits, ld, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index);
-  else
-    hipLaunchKernelGGL(token_logprobs_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t*)logits, ld, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index);
+  if (dtype == S2T_F32) launch_fwd<float, 256>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
+  else launch_fwd<bf16_t, 256>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
   return S2T_LAUNCH_CHECK();
 }
 
