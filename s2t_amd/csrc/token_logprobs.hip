@@ -46,8 +46,8 @@ __device__ __forceinline__ bool before(Best a, Best b) { return a.v > b.v || (a.
 
 // One workgroup to a row, one pass: every thread keeps the statistics of its vectors (relative to its own running maximum, moved once
 // for each NB vectors) and, for the alternatives, the maximum of its raw logits.  The top-th largest of the 64 maxima of four threads
-// each bounds the alternatives from below, since as many columns reach it; the threads that do collect their columns that reach it
-// (read once more, from the caches), usually hardly more than `top`, and one wave ranks them by (logit, column).  Rows with more than
+// each bounds the alternatives from below, since as many columns reach it; the columns of the threads that reach it are read once more
+// (from the caches, dealt to all threads), those that reach it, usually hardly more than `top`, are collected and ranked by (logit, column).  Rows with more than
 // CAND such columns (ties without end) are ranked one column after the other instead.
 constexpr int CAND = 512;
 template <typename T, int THREADS, bool TOP, bool ENTROPY>
@@ -77,10 +77,12 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
   const int nvec = V / E, tail = nvec * E + tid;  // thread `tid`: vectors tid, tid + THREADS .., and one of the V % E last columns
   Stats st{-INFINITY, 0.f, 0.f};
   float most = -INFINITY;
-  auto take = [&](const float* x, int n) __attribute__((always_inline)) {
+  // N columns: the maximum first, so that the sums are moved once for all of them
+  auto take = [&](const auto& x) __attribute__((always_inline)) {
+    constexpr int N = sizeof(x) / sizeof(float);
     float hi = x[0];
 #pragma unroll
-    for (int e = 1; e < n; ++e) hi = fmaxf(hi, x[e]);
+    for (int e = 1; e < N; ++e) hi = fmaxf(hi, x[e]);
     if (TOP) most = fmaxf(most, hi);
     hi *= c2;
     if (hi > st.m) {
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
     }
     const float ref = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
-    for (int e = 0; e < n; ++e) {
+    for (int e = 0; e < N; ++e) {
       const float d = fmaf(x[e], c2, -ref), p = exp2_(d);
       st.s += p;
       if (ENTROPY) st.t = fmaf(p, fmaxf(d, -1e30f), st.t);  // (a column of -inf: 0 * -1e30)
@@ -101,27 +103,38 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
     Vec buf[NB];
 #pragma unroll
     for (int u = 0; u < NB; ++u) buf[u] = *reinterpret_cast<const Vec*>(row + (int64_t)min(v0 + u * THREADS, nvec - 1) * E);
+    float x[NB * E];
 #pragma unroll
-    for (int u = 0; u < NB; ++u)
-      if (v0 + u * THREADS < nvec) {
-        float x[E];
-        unpack<T>(buf[u], x);
-        take(x, E);
-      }
+    for (int u = 0; u < NB; ++u) {
+      if (v0 + u * THREADS >= nvec)  // -inf: adds nothing
+#pragma unroll
+        for (int q = 0; q < 4; ++q) buf[u].w[q] = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+      float y8[E];
+      unpack<T>(buf[u], y8);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[u * E + e] = y8[e];
+    }
+    take(x);
   }
   if (tail < V) {
-    const float x = ld_as_f32<T>(row + tail);
-    take(&x, 1);
+    const float x[1] = {ld_as_f32<T>(row + tail)};
+    take(x);
   }
   __shared__ Stats part[WAVES];
   __shared__ float maxima[TOP ? THREADS : 1];
   __shared__ Best cand[TOP ? CAND : 1];
-  __shared__ int n_cand;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) st = merged(st, Stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)});
+  __shared__ int winner[TOP ? THREADS : 1];
+  __shared__ int n_cand, n_win;
+  {  // of a wave: the common maximum, then sums
+    const float m = wave_max(st.m), ref = m == -INFINITY ? 0.f : m, d = st.m - ref, f = exp2_(d);
+    const float sum = wave_sum(st.s * f);
+    st.t = ENTROPY ? wave_sum(f == 0.f ? 0.f : f * (st.t + st.s * d)) : 0.f;
+    st.s = sum;
+    st.m = m;
+  }
   if (lane == 0) part[w] = st;
   if (TOP) maxima[tid] = most;
-  if (tid == 0) n_cand = 0;
+  if (tid == 0) n_cand = n_win = 0;
   __syncthreads();
   st = part[0];
 #pragma unroll
@@ -134,30 +147,33 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
     if (logprob) logprob[r] = (uint64_t)y < (uint64_t)V ? score(ld_as_f32<T>(row + y)) : __builtin_nanf("");
   }
   if constexpr (TOP) {
-    // the bound: every wave finds it for itself
-    float bound = maxima[lane];
+    // the bound: the largest of the 64 that `top` of them reach; every wave finds it for itself
+    float mine = maxima[lane];
 #pragma unroll
-    for (int q = 1; q < WAVES; ++q) bound = fmaxf(bound, maxima[q * 64 + lane]);
-    float left = bound;
-    for (int k = 0; k < top; ++k) {
-      bound = wave_max(left);
-      const uint64_t who = __ballot(left == bound);
-      if (lane == (who ? __builtin_ctzll(who) : 0)) left = -INFINITY;
-    }
-    if (most >= bound) {
-      auto offer = [&](float v, int i) {
-        if (v >= bound) {
-          const int at = atomicAdd(&n_cand, 1);
-          if (at < CAND) cand[at] = Best{v, i};
-        }
-      };
-      for (int v = tid; v < nvec; v += THREADS) {
+    for (int q = 1; q < WAVES; ++q) mine = fmaxf(mine, maxima[q * 64 + lane]);
+    int reach = 0;
+#pragma unroll
+    for (int q = 0; q < 64; ++q) reach += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), q)) >= mine ? 1 : 0;
+    const float bound = wave_max(reach >= top ? mine : -INFINITY);
+    auto offer = [&](float v, int i) {
+      if (v >= bound) {
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < CAND) cand[at] = Best{v, i};
+      }
+    };
+    if (most >= bound) winner[atomicAdd(&n_win, 1)] = tid;
+    if (tail < V) offer(ld_as_f32<T>(row + tail), tail);
+    __syncthreads();
+    // the vectors of the threads that reach it, dealt to all threads: each of them one load
+    const int of_one = (nvec + THREADS - 1) / THREADS, all = n_win * of_one;
+    for (int q = tid; q < all; q += THREADS) {
+      const int v = winner[q / of_one] + q % of_one * THREADS;
+      if (v < nvec) {
         float x[E];
         unpack<T>(*reinterpret_cast<const Vec*>(row + (int64_t)v * E), x);
 #pragma unroll
         for (int e = 0; e < E; ++e) offer(x[e], v * E + e);
       }
-      if (tail < V) offer(ld_as_f32<T>(row + tail), tail);
     }
     __syncthreads();
     const int n = n_cand;

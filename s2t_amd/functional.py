@@ -2356,14 +2356,23 @@ class TokenLogprobsFn(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logprob, g_entropy, g_top, _):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("token_logprobs is differentiable once")
         logits, tokens, lse, entropy, top_idx = ctx.saved_tensors
         ignore_index, inv_temp, top = ctx.args
         if g_logprob is None and g_entropy is None and g_top is None:
-            return (None,) * 6
-        dl = torch.empty(logits.shape[0], _pad8(logits.shape[1]), dtype=logits.dtype, device=logits.device)[:, :logits.shape[1]]
-        g_logprob, g_entropy, g_top = (g.contiguous() if g is not None else None for g in (g_logprob, g_entropy, g_top))
+            return None, None, None, None, None, None
+        rows, V = logits.shape
+        dl = torch.empty(rows, _pad8(V), dtype=logits.dtype, device=logits.device)
+        if V % 8:
+            dl = dl[:, :V]
+        if g_logprob is not None and not g_logprob.is_contiguous():
+            g_logprob = g_logprob.contiguous()
+        if g_entropy is not None and not g_entropy.is_contiguous():
+            g_entropy = g_entropy.contiguous()
+        if g_top is not None and not g_top.is_contiguous():
+            g_top = g_top.contiguous()
         K.token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_idx, dl)
         return dl, None, None, None, None, None
 

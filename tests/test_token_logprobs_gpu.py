@@ -211,6 +211,14 @@ def test_an_empty_batch_and_partial_gradients():
         assert float((dx.cpu().double() - grad).abs().max()) <= 40 * _ep(x.cpu(), 1.0)  # |upstream| <= 4 in four terms, H <= log 77 < 5
 
 
+def test_a_second_derivative_is_refused():
+    x, g = _logits(2, 9, torch.float32, 1)
+    leaf = x.detach().requires_grad_()
+    r = Fn.token_logprobs(leaf, torch.zeros(2, dtype=torch.int64, device=DEV))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(r.logprob.sum(), leaf, create_graph=True)
+
+
 def test_two_runs_are_equal_and_a_graph_replays():
     x, g = _logits(300, 10000, torch.bfloat16, 8)
     tokens = torch.randint(0, 10000, (300,), generator=g).to(DEV)
