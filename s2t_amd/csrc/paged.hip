@@ -7,6 +7,10 @@
 
 namespace {
 
+// Table, lens, cu and the like are uniform over a wave and only read here: through the constant address space they come by scalar loads,
+// which do not queue behind the vector loads of keys and values.
+typedef const __attribute__((address_space(4))) int32_t* Entries;
+
 // place -> element offset of (page, place in page), or -1 where the table does not lead to a page
 struct Pages {
   const int32_t* table;  // this sequence's row
@@ -15,7 +19,7 @@ struct Pages {
   __device__ __forceinline__ int64_t at(int place) const {
     const int i = place >> shift;
     if (place < 0 || i >= n_table) return -1;
-    const int p = table[i];
+    const int p = ((Entries)table)[i];
     return (uint32_t)p < (uint32_t)num_pages ? p * sp + (place & mask) * sr : -1;
   }
 };
@@ -27,14 +31,15 @@ struct Span {
   int row0, n, len;
 };
 __device__ __forceinline__ Span span_of(const s2t_paged_args& a, int b) {
-  const int r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
-  return {r0, max(r1 - r0, 0), a.lens[b]};
+  const Entries cu = (Entries)a.cu;
+  const int r0 = min(max(cu[b], 0), a.N), r1 = min(max(cu[b + 1], 0), a.N);
+  return {r0, max(r1 - r0, 0), ((Entries)a.lens)[b]};
 }
 
 // ---- append -----------------------------------------------------------------------------------------------------------------
-// A wave takes TOKENS new tokens of a sequence; its lanes go over the units of a token (16 bytes that pass, or two times 16 that turn
-// together: first all of k, then v, then q), each for all of its tokens at once, so that TOKENS loads are on their way before the first
-// store and what a unit is has to be worked out once.  Where the tokens go comes by scalar loads.
+// A wave takes a new token; its lanes go over the token's units: 16 bytes that pass, or two times 16 that turn together, first all of k, then
+// v, then q.  (Bound by memory, and kept busy by many small waves: two, four and eight tokens to a wave, with as many loads of each
+// lane on their way, were slower, 48, 57 and 63 us against 42 for 16 900 tokens of 4 + 4 + 16 heads x 128 in bf16, 210 MB: 5.0 TB/s.)
 template <typename T>
 struct Turned {
   static constexpr int E = 16 / (int)sizeof(T);
@@ -71,58 +76,40 @@ struct Turned {
   }
 };
 
-template <typename T, int TOKENS>
+template <typename T>
 __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args a, const int shift, const uint32_t by_units, const uint32_t by_vecs) {
   constexpr int E = Turned<T>::E;
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i0 = (blockIdx.x * 4 + wave) * TOKENS;
+  const int b = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = blockIdx.x * 4 + wave;
   const Span s = span_of(a, b);
-  const int n = min(s.n, a.max_new);
-  if (i0 >= n) return;
-  const Pages pages = pages_of(a, shift, b);
+  if (i >= min(s.n, a.max_new)) return;
   const int rot = a.rotary ? a.rot_dim : 0, half = rot / 2;
   const int pairs = half / E, units = pairs + (a.dk - rot) / E, vecs = a.dk / E;
   const int nk = a.kv_heads * units, nv = a.kv_heads * vecs, nq = a.q ? a.q_heads * units : 0;
-  int64_t to[TOKENS], from[TOKENS];
-  const float* cs[TOKENS];
-  bool known[TOKENS], stored[TOKENS];
-#pragma unroll
-  for (int j = 0; j < TOKENS; ++j) {
-    const int i = min(i0 + j, n - 1), t = s.row0 + i, place = s.len - s.n + i;
-    to[j] = pages.at(place);
-    const int row = a.rows ? a.rows[t] : t, pos = a.positions ? a.positions[t] : place;
-    const bool there = !a.rows || (uint32_t)row < (uint32_t)a.src_rows;
-    from[j] = there ? row : 0;
-    known[j] = (uint32_t)pos < (uint32_t)a.rotary_positions;
-    cs[j] = a.rotary + (int64_t)(known[j] ? pos : 0) * rot;
-    stored[j] = i0 + j < n && to[j] >= 0 && there;
-  }
-  for (int u = lane; u < nk + nv + nq; u += 64) {
+  const int t = s.row0 + i, place = s.len - s.n + i;
+  const int64_t to = pages_of(a, shift, b).at(place);
+  const int row = a.rows ? ((Entries)a.rows)[t] : t, pos = a.positions ? ((Entries)a.positions)[t] : place;
+  const bool there = !a.rows || (uint32_t)row < (uint32_t)a.src_rows, stored = to >= 0 && there;
+  const bool known = (uint32_t)pos < (uint32_t)a.rotary_positions;
+  const float* cs = a.rotary + (int64_t)(known ? pos : 0) * rot;
+  for (int u = threadIdx.x & 63; u < nk + nv + nq; u += 64) {
     // what this unit is
     const bool is_v = u >= nk && u < nk + nv, is_q = u >= nk + nv;
     const int w = is_q ? u - nk - nv : is_v ? u - nk : u, per = is_v ? vecs : units;
     const int h = per == 1 ? w : (int)__umulhi((uint32_t)w, is_v ? by_vecs : by_units), c = w - h * per;
     const bool pair = !is_v && c < pairs;
-    const int col = is_v ? c * E : pair ? c * E : rot + (c - pairs) * E;
-    const T* src = (is_v ? (const T*)a.v + h * a.v_sh : is_q ? (const T*)a.q + h * a.q_sh : (const T*)a.k + h * a.k_sh) + col;
-    T* dst = (is_v ? (T*)a.v_pages + h * a.p_sh : is_q ? (T*)a.q_out + h * a.qo_sh : (T*)a.k_pages + h * a.p_sh) + col;
-    const int64_t src_step = is_v ? a.v_st : is_q ? a.q_st : a.k_st;
-    uint4 x[TOKENS], y[TOKENS];
-#pragma unroll
-    for (int j = 0; j < TOKENS; ++j) {
-      const T* p = src + (is_q ? (int64_t)(s.row0 + min(i0 + j, n - 1)) : from[j]) * src_step;
-      x[j] = *reinterpret_cast<const uint4*>(p);
-      if (pair) y[j] = *reinterpret_cast<const uint4*>(p + half);
+    const int col = is_v || pair ? c * E : rot + (c - pairs) * E;
+    const T* src = (is_v ? (const T*)a.v + row * a.v_st + h * a.v_sh : is_q ? (const T*)a.q + t * a.q_st + h * a.q_sh : (const T*)a.k + row * a.k_st + h * a.k_sh) + col;
+    T* dst = (is_v ? (T*)a.v_pages + to + h * a.p_sh : is_q ? (T*)a.q_out + t * a.qo_st + h * a.qo_sh : (T*)a.k_pages + to + h * a.p_sh) + col;
+    if (!is_q && !there) continue;
+    uint4 x = *reinterpret_cast<const uint4*>(src), y = x;
+    if (pair) {
+      y = *reinterpret_cast<const uint4*>(src + half);
+      Turned<T>::turn(x, y, cs + c * E, half, known);
     }
-#pragma unroll
-    for (int j = 0; j < TOKENS; ++j) {
-      if (pair) Turned<T>::turn(x[j], y[j], cs[j] + c * E, half, known[j]);
-      T* p = dst + (is_q ? (int64_t)(s.row0 + i0 + j) * a.qo_st : to[j]);
-      if (is_q ? i0 + j < n : stored[j]) {
-        *reinterpret_cast<uint4*>(p) = x[j];
-        if (pair) *reinterpret_cast<uint4*>(p + half) = y[j];
-      }
-    }
+    if (!is_q && !stored) continue;
+    *reinterpret_cast<uint4*>(dst) = x;
+    if (pair) *reinterpret_cast<uint4*>(dst + half) = y;
   }
 }
 
@@ -249,8 +236,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   auto find = [&](int key0) {
     Where w;
     if constexpr (BIG) {
-      // (the table through scalar loads: as vector loads they would wait behind the values that are on their way)
-      const auto entries = (const __attribute__((address_space(4))) int32_t*)table;
+      const Entries entries = (Entries)table;
       const int i0 = key0 >> shift, i1 = (key0 + 16) >> shift;
       const int p0 = i0 < a.table_pages ? entries[i0] : -1, p1 = i1 < a.table_pages ? entries[i1] : -1;
       const bool ok0 = (uint32_t)p0 < (uint32_t)a.num_pages, ok1 = (uint32_t)p1 < (uint32_t)a.num_pages;
@@ -707,12 +693,9 @@ extern "C" int s2t_paged_kv_append(const s2t_paged_args* a, void* stream) {
   const int e = a->dtype == S2T_F32 ? 4 : 8, rot = a->rotary ? a->rot_dim : 0, units = rot / 2 / e + (a->dk - rot) / e, vecs = a->dk / e;
   if ((int64_t)std::max(a->q_heads, a->kv_heads) * vecs * vecs >= (1ll << 31)) return S2T_ERR_UNSUPPORTED;  // (divisions by reciprocals)
   const auto by = [](int n) { return n > 1 ? (uint32_t)((1ull << 32) / n + 1) : 0u; };
-  // four tokens to a wave where that still leaves the chip its waves
-  const bool many = (int64_t)a->max_new * a->B >= 16384;
-  const dim3 grid((unsigned)((a->max_new + (many ? 15 : 3)) / (many ? 16 : 4)), (unsigned)a->B);
-  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs)); };
-  if (a->dtype == S2T_F32) many ? go(paged_append_kernel<float, 4>) : go(paged_append_kernel<float, 1>);
-  else many ? go(paged_append_kernel<bf16_t, 4>) : go(paged_append_kernel<bf16_t, 1>);
+  const dim3 grid((unsigned)((a->max_new + 3) / 4), (unsigned)a->B);
+  if (a->dtype == S2T_F32) hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs));
+  else hipLaunchKernelGGL(paged_append_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs));
   return S2T_LAUNCH_CHECK();
 }
 
