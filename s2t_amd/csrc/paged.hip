@@ -163,7 +163,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 
 // T: type of the cache; DK: head_dim rounded up to 32, 64, 128 or 256; BIG: a half tile of 16 keys lies in one page
 template <typename T, int DK, int MT, bool BIG>
-__global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int n_tiles, const int n_split,
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int n_tiles, const int n_split,
                                                               const float c2, const int flip, float* __restrict__ part) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = DK / 16;          // 16-column tiles of the output
@@ -211,8 +211,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   for (int mt = 0; mt < MT; ++mt) {
     const int row = row_base + mt * 16 + c;
     const bool live = row < rc.rows;
-    tok[mt] = live ? row / group : 0;
-    const T* q = (const T*)a.q + (int64_t)(sp.row0 + tok[mt]) * a.q_st + (int64_t)(h * group + (live ? row % group : 0)) * a.q_sh;
+    tok[mt] = !live ? 0 : group == 1 ? row : row / group;
+    const T* q = (const T*)a.q + (int64_t)(sp.row0 + tok[mt]) * a.q_st + (int64_t)(h * group + (live ? row - tok[mt] * group : 0)) * a.q_sh;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
       const int col = (ks * 4 + g) * KE;
@@ -233,35 +233,43 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
     int64_t row;           // !BIG: offset of key key0 + (lane & 31)
     uint32_t exist;        // bit of each of the 32 keys: it lies on a page
   };
-  auto find = [&](int key0) {
+  // (the entries of the tile after the next are asked for a tile ahead; an index beyond the table is read at its end and then left out)
+  struct Pair {
+    int p0, p1;
+  };
+  auto entries = [&](int key0) {
+    const Entries e = (Entries)table;
+    const int last = a.table_pages - 1;
+    if constexpr (BIG) return Pair{e[min(key0 >> shift, last)], e[min((key0 + 16) >> shift, last)]};
+    else return Pair{table[min((key0 + (lane & 31)) >> shift, last)], 0};
+  };
+  auto find = [&](int key0, Pair e) {
     Where w;
     if constexpr (BIG) {
-      const Entries entries = (Entries)table;
-      const int i0 = key0 >> shift, i1 = (key0 + 16) >> shift;
-      const int p0 = i0 < a.table_pages ? entries[i0] : -1, p1 = i1 < a.table_pages ? entries[i1] : -1;
-      const bool ok0 = (uint32_t)p0 < (uint32_t)a.num_pages, ok1 = (uint32_t)p1 < (uint32_t)a.num_pages;
-      w.half0 = (ok0 ? p0 * a.p_sp : 0) + (int64_t)(key0 & mask) * sr;
-      w.half1 = (ok1 ? p1 * a.p_sp : 0) + (int64_t)((key0 + 16) & mask) * sr;
+      const bool ok0 = (uint32_t)e.p0 < (uint32_t)a.num_pages && (key0 >> shift) < a.table_pages;
+      const bool ok1 = (uint32_t)e.p1 < (uint32_t)a.num_pages && ((key0 + 16) >> shift) < a.table_pages;
+      w.half0 = (ok0 ? e.p0 : 0) * a.p_sp + (int64_t)(key0 & mask) * sr;
+      w.half1 = (ok1 ? e.p1 : 0) * a.p_sp + (int64_t)((key0 + 16) & mask) * sr;
       w.exist = (ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u);
     } else {
-      const int key = key0 + (lane & 31), i = key >> shift;
-      const int p = i < a.table_pages ? table[i] : -1;
-      const bool ok = (uint32_t)p < (uint32_t)a.num_pages;
-      w.row = ok ? p * a.p_sp + (int64_t)(key & mask) * sr : 0;
+      const int key = key0 + (lane & 31);
+      const bool ok = (uint32_t)e.p0 < (uint32_t)a.num_pages && (key >> shift) < a.table_pages;
+      w.row = ok ? e.p0 * a.p_sp + (int64_t)(key & mask) * sr : 0;
       w.exist = (uint32_t)__ballot(ok);
     }
     return w;
   };
-  // (BIG: a scalar base and one 32-bit offset of the lane for all loads of a tile)
-  const uint32_t koff = (uint32_t)(c * sr) * (uint32_t)sizeof(T), voff = (uint32_t)(4 * g * sr + vcol) * (uint32_t)sizeof(T);
+  // BIG: offsets of the lane from a tile's base that hold for every tile
+  uint32_t koff[NK];
+#pragma unroll
+  for (int ks = 0; ks < NK; ++ks) koff[ks] = (uint32_t)((BIG ? c * sr : 0) + min((ks * 4 + g) * KE, d - KE)) * (uint32_t)sizeof(T);
+  const uint32_t voff = (uint32_t)((BIG ? 4 * g * sr : 0) + vcol) * (uint32_t)sizeof(T);
   auto load_k = [&](const Where& w, u32x4 (&kf)[2][NK]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* p;
-      if constexpr (BIG) p = (const char*)(kpool + (t ? w.half1 : w.half0)) + koff;
-      else p = (const char*)(kpool + (int64_t)__shfl(w.row, 16 * t + c, 64));
+      const char* p = (const char*)(kpool + (BIG ? (t ? w.half1 : w.half0) : (int64_t)__shfl(w.row, 16 * t + c, 64)));
 #pragma unroll
-      for (int ks = 0; ks < NK; ++ks) kf[t][ks] = *reinterpret_cast<const u32x4*>(p + (uint32_t)min((ks * 4 + g) * KE, d - KE) * (uint32_t)sizeof(T));
+      for (int ks = 0; ks < NK; ++ks) kf[t][ks] = *reinterpret_cast<const u32x4*>(p + koff[ks]);
     }
     if (d != DK) {
 #pragma unroll
@@ -275,18 +283,16 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
   auto load_v = [&](const Where& w, uint32_t (&vr)[8][VW]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const char* p;
-      if constexpr (BIG) p = (const char*)(vpool + (e >> 2 ? w.half1 : w.half0) + (e & 3) * sr) + voff;
-      else p = (const char*)(vpool + vcol + (int64_t)__shfl(w.row, 16 * (e >> 2) + 4 * g + (e & 3), 64));
-      if constexpr (VB == 4) vr[e][0] = *reinterpret_cast<const uint32_t*>(p);
+      const char* p = (const char*)(vpool + (BIG ? (e >> 2 ? w.half1 : w.half0) + (e & 3) * sr : (int64_t)__shfl(w.row, 16 * (e >> 2) + 4 * g + (e & 3), 64)));
+      if constexpr (VB == 4) vr[e][0] = *reinterpret_cast<const uint32_t*>(p + voff);
       else if constexpr (VB == 8) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p + voff);
         vr[e][0] = x.x;
         vr[e][1] = x.y;
       } else {
 #pragma unroll
         for (int q = 0; q < VW / 4; ++q) {
-          const u32x4 x = reinterpret_cast<const u32x4*>(p)[q];
+          const u32x4 x = reinterpret_cast<const u32x4*>(p + voff)[q];
           vr[e][4 * q] = x.x;
           vr[e][4 * q + 1] = x.y;
           vr[e][4 * q + 2] = x.z;
@@ -313,14 +319,18 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
     int key0 = split * chunk + 32 * wave;
     Where w;
     uint32_t vr[8][VW];
+    Pair e{0, 0};
     if (!careful && key0 < k_hi) {
-      w = find(key0);
+      w = find(key0, entries(key0));
       load_k(w, kf);
       load_v(w, vr);
+      e = entries(key0 + 128);
     }
-    while (key0 < k_hi) {  // (a tile's keys and values are both on their way while the tile before it is worked on)
+    // A tile's keys and values are both on their way while the tile before it is worked on.  (The last tile asks for itself once more
+    // instead of for nothing: behind a branch the compiler would have every wait for keys wait for the values as well.)
+    while (key0 < k_hi) {
       if constexpr (careful) {  // (with nothing on its way, and the corrections last: this round is not to need more registers)
-        w = find(key0);
+        w = find(key0, entries(key0));
         load_k(w, kf);
       }
       // scores of all rows, then the next tile's keys can be fetched
@@ -344,9 +354,10 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
       const Where now = w;
       const int next = key0 + 128;
       if constexpr (careful) load_v(now, vr);
-      else if (next < k_hi) {
-        w = find(next);
+      else {
+        if (next < k_hi) w = find(next, e);
         load_k(w, kf);
+        e = entries(next + 128);
       }
       __builtin_amdgcn_sched_barrier(0);
       // keys of this tile that exist, and whether every row sees all of them
@@ -354,10 +365,11 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
       const bool whole = exist == 0xffffffffu && key0 + 32 <= all_see;
       uint32_t vis[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        vis[mt] = 0xffffffffu;
-        if (!whole) {
-          const int j0 = key0 - rc.prefix;
+      for (int mt = 0; mt < MT; ++mt) vis[mt] = 0xffffffffu;
+      if (!whole) {
+        const int j0 = key0 - rc.prefix;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
           uint32_t x;
           if (a.tree) x = tree_window(a.tree + (int64_t)(sp.row0 + tok[mt]) * a.tree_stride, a.tree_words, j0) | low_bits(-j0);
           else x = low_bits(tok[mt] - j0 + 1);
@@ -369,18 +381,36 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
             for (int r = 0; r < 4; ++r)
               if (!((mine >> (16 * t + r)) & 1)) s[mt][t][r] = -INFINITY;
         }
-        // reference
-        const float top = c2 * fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
-                                     fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
-        if (__any(top > m[mt] + 8.f)) {
-          const float mn = fmaxf(m[mt], s2t_xmax<16>(s2t_xmax<32>(top)));
-          const float fade = mn == -INFINITY ? 1.f : exp2_(m[mt] - mn);
+      }
+      // exponents against the references so far; one vote for all row tiles whether any of these has to move
+      bool grow = false;
+      float top[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[mt][t][r] = fmaf(s[mt][t][r], c2, -ref);
+        top[mt] = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                        fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
+        grow = grow || top[mt] > (m[mt] == -INFINITY ? -INFINITY : 8.f);
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+          const float mn = fmaxf(m[mt], ref + s2t_xmax<16>(s2t_xmax<32>(top[mt])));
+          const float move = mn == -INFINITY ? 0.f : ref - mn, fade = mn == -INFINITY ? 1.f : exp2_(m[mt] - mn);
           m[mt] = mn;
           l[mt] *= fade;
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] *= fade;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[mt][t] += move;
         }
       }
+      __builtin_amdgcn_s_setprio(1);  // (the wave that has its scores before the one that waits for keys: prompts 69.7 -> 66.7 us)
       // values: operand A of O^T
       if (exist != 0xffffffffu) {  // what lies behind the end is not to be multiplied with anything
 #pragma unroll
@@ -407,21 +437,17 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             va[dt][q] = __builtin_amdgcn_perm(vr[2 * q + 1][dt >> 1], vr[2 * q][dt >> 1], dt & 1 ? 0x07060302u : 0x05040100u);
-        if (!careful && next < k_hi) load_v(w, vr);
+        if constexpr (!careful) load_v(w, vr);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
-        float p[2][4], sum = 0.f;
+        float p[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            p[t][r] = exp2_(fmaf(s[mt][t][r], c2, -ref));
-            sum += p[t][r];
-          }
-        l[mt] += sum;
+          for (int r = 0; r < 4; ++r) p[t][r] = exp2_(s[mt][t][r]);
+        l[mt] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
         if constexpr (BF) {
           u32x4 hi, lo;
 #pragma unroll
@@ -476,8 +502,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
         }
         __builtin_amdgcn_wave_barrier();
       }
-      if constexpr (!BF && !careful)
-        if (next < k_hi) load_v(w, vr);
+      __builtin_amdgcn_s_setprio(0);
+      if constexpr (!BF && !careful) load_v(w, vr);
       key0 = next;
     }
   };
@@ -527,7 +553,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const s2t_paged_ar
     }
     const int row = row_base + mt * 16 + c, col = (4 * g + wave) * NDT;
     if (row >= rc.rows || col >= d) continue;
-    const int t = sp.row0 + row / group, hq = h * group + row % group;
+    const int i = tok[mt], t = sp.row0 + i, hq = h * group + row - i * group;
     if (used == 1) {
       const float inv = top == -INFINITY ? 0.f : 1.f / total;
       T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
