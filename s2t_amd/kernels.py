@@ -1022,26 +1022,19 @@ def _call_on(device, name, *args):
         L.check(status, name)
 
 
-def paged_kv_append(device, *fields):
-    """s2t_paged_kv_append; ``fields``: those of s2t_paged_args (include/s2t_hip.h) in order, the attention's left out."""
-    _call_on(device, "s2t_paged_kv_append", L.PAGED_ARGS.pack(*fields, *_NO_ATTENTION))
-
-
-_NO_ATTENTION = (0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0)
-_NO_APPEND = (0, 0, 0, 0, 0, 0, 0, 0, 0)
 PAGED_ONE_RANGE = 1023  # up to so many places of a sequence the attention needs no workspace (csrc/paged.hip, cut_of)
 
 
-def paged_attention(device, cache, q, out_to_scale):
-    """s2t_paged_attention; the workspace comes from the allocator (a captured graph keeps its own).  ``cache``: the fields up to cu,
-    ``q``: its address and strides, ``out_to_scale``: out .. scale."""
-    head = cache + (0, 0, 0, 0, 0, 0) + q + _NO_APPEND + out_to_scale
-    args = L.PAGED_ARGS.pack(*head, 0, 0)
-    if cache[8] * cache[9] > PAGED_ONE_RANGE:
-        n = L.lib().s2t_paged_attention_ws_bytes(args)
-        if n > 0:
-            ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", device))
-            args = L.PAGED_ARGS.pack(*head, ws.data_ptr(), n)
+def paged_kv_append(device, args):
+    """s2t_paged_kv_append; ``args``: L.PAGED_ARGS.pack of s2t_paged_args' fields (include/s2t_hip.h)."""
+    _call_on(device, "s2t_paged_kv_append", args)
+
+
+def paged_attention_ws_bytes(args):
+    return L.lib().s2t_paged_attention_ws_bytes(args)
+
+
+def paged_attention(device, args):
     _call_on(device, "s2t_paged_attention", args)
 
 

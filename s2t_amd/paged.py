@@ -27,6 +27,7 @@ _I32 = torch.int32
 
 
 _NONE3 = (0, 0, 0)
+_NO_KV, _NO_APPEND, _NO_ATTENTION = (0,) * 6, (0,) * 9, (0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0)  # fields of s2t_paged_args that a call leaves out
 
 
 def _refuse(what):
@@ -83,20 +84,29 @@ def _rows(name, t, heads, like, n=None):
     return t.data_ptr(), stride[0], stride[1]
 
 
+def _like(q):
+    """-> a new tensor of q's shape, its address and strides."""
+    t = torch.empty_like(q)
+    stride = t.stride()
+    return t, (t.data_ptr(), stride[0], stride[1])
+
+
 def _index(name, t, n):
     if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         _refuse("%s must be int32 [%d], contiguous" % (name, n))
     return t.data_ptr()
 
 
-def _device(*tensors):
-    """-> index of the one device that all of them (None aside) live on."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev or dev < 0:
-            L.require_cuda(*tensors)
-            _refuse("tensors on several devices: %s" % ", ".join(str(t.device) for t in tensors if t is not None))
-    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors if t is not None]):
+def _device(k_pages, v_pages, page_table, lens, cu, x, *others):
+    """-> index of the one device that all of them (None aside) live on; ``x``: the rows that come first."""
+    dev = k_pages.get_device()
+    if not (dev == v_pages.get_device() == page_table.get_device() == lens.get_device() == cu.get_device() == x.get_device()) or dev < 0 \
+            or [1 for t in others if t is not None and t.get_device() != dev]:
+        tensors = (k_pages, v_pages, page_table, lens, cu, x) + others
+        L.require_cuda(*tensors)
+        _refuse("tensors on several devices: %s" % ", ".join(str(t.device) for t in tensors if t is not None))
+    if (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad or [1 for t in others if t is not None and t.requires_grad]) \
+            and torch.is_grad_enabled():
         raise RuntimeError("the paged cache is inference only: wrap the decoder in torch.no_grad()")
     return dev
 
@@ -119,9 +129,7 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
         if rows is not None:
             _refuse("q cannot be turned together with a selection of rows")
         qf = _rows("q", q, None, k_pages, N)
-        if q_out is None:
-            q_out = torch.empty_like(q)
-        of = _rows("q_out", q_out, cache[4], k_pages, N)
+        q_out, of = _like(q) if q_out is None else (q_out, _rows("q_out", q_out, cache[4], k_pages, N))
     elif q_out is not None:
         _refuse("q_out without q")
     turn = _NONE3
@@ -133,8 +141,8 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
         turn = (rotary.data_ptr(),) + tuple(rotary.shape)
     at = _index("positions", positions, N) if positions is not None else 0
     pick = _index("rows", rows, N) if rows is not None else 0
-    dev = _device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out)
-    K.paged_kv_append(dev, *cache, *kf, *vf, *qf, *of, *turn, at, pick, k.shape[0])
+    K.paged_kv_append(_device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out),
+                      L.PAGED_ARGS.pack(*cache, *kf, *vf, *qf, *of, *turn, at, pick, k.shape[0], *_NO_ATTENTION))
     return q_out
 
 
@@ -154,13 +162,18 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
         if tree.dtype is not torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
             _refuse("tree must be int64 [%d, words] with contiguous rows, got %s %s" % (N, tuple(tree.shape), tree.dtype))
         bits = (tree.data_ptr(), tree.stride(0), tree.shape[1])
-    if out is None:
-        out = torch.empty_like(q)
-    of = _rows("out", out, Hq, k_pages, N)
+    out, of = _like(q) if out is None else (out, _rows("out", out, Hq, k_pages, N))
     dev = _device(k_pages, v_pages, page_table, lens, cu, q, tree, out)
     lse, to_lse = None, 0
     if return_lse:
         lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device)
         to_lse = lse.data_ptr()
-    K.paged_attention(dev, cache, qf, of + (to_lse,) + bits + (d ** -0.5 if scale is None else float(scale),))
+    tail = (to_lse, *bits, d ** -0.5 if scale is None else float(scale))
+    args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, 0, 0)
+    if cache[8] * cache[9] > K.PAGED_ONE_RANGE:
+        n = K.paged_attention_ws_bytes(args)
+        if n > 0:  # from the allocator: a captured graph keeps its own, another stream gets another
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, ws.data_ptr(), n)
+    K.paged_attention(dev, args)
     return (out, lse) if return_lse else out
