@@ -832,6 +832,7 @@ typedef struct s2t_paged_args {
   int64_t tree_stride;
   int32_t tree_words;     /* words of a row that exist; new tokens beyond 64 * tree_words are not seen */
   float scale;
+  int32_t memory;         /* != 0: lens counts a memory without the new tokens, all of which see all of it (encoder-decoder attention; no tree) */
   void* ws;               /* s2t_paged_attention_ws_bytes(args) bytes, 16-byte aligned; contents undefined before and after */
   int64_t ws_bytes;
 } s2t_paged_args;

@@ -118,8 +118,8 @@ class RowblockArgs(C.Structure):
 # costs 0.7 us where filling a ctypes structure field by field costs 5.
 PAGED_FIELDS = ("dtype B N max_new q_heads kv_heads dk num_pages page_size table_pages k_pages v_pages p_sp p_sh p_sr page_table table_stride "
                 "lens cu k k_st k_sh v v_st v_sh q q_st q_sh q_out qo_st qo_sh rotary rotary_positions rot_dim positions rows src_rows out o_st "
-                "o_sh lse tree tree_stride tree_words scale ws ws_bytes").split()
-PAGED_ARGS = struct.Struct("@10i PPqqq Pq PP Pqq Pqq Pqq Pqq Pii PPi Pqq P Pqi f Pq")
+                "o_sh lse tree tree_stride tree_words scale memory ws ws_bytes").split()
+PAGED_ARGS = struct.Struct("@10i PPqqq Pq PP Pqq Pqq Pqq Pqq Pii PPi Pqq P Pqi f i Pq")
 
 
 _CTYPE = {"int": C.c_int, "int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float, "uint32_t": C.c_uint32}

@@ -147,7 +147,7 @@ __device__ __forceinline__ Reach reach_of(const s2t_paged_args& a, const Span& s
   Reach r;
   r.rows = min(s.n, a.max_new) * group;
   r.len = min(s.len, a.table_pages << shift);
-  r.prefix = s.len - s.n;
+  r.prefix = a.memory ? r.len : s.len - s.n;
   const int last = (min(row_base + tile_rows, r.rows) - 1) / group;
   r.kend = a.tree ? r.len : min(r.len, r.prefix + last + 1);
   return r;
@@ -734,7 +734,7 @@ extern "C" int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* a) {
 
 extern "C" int s2t_paged_attention(const s2t_paged_args* a, void* stream) {
   if (int bad = paged_args_bad(a)) return bad;
-  if ((a->tree && a->tree_words <= 0) || !(a->scale == a->scale)) return S2T_ERR_ARG;
+  if ((a->tree && (a->tree_words <= 0 || a->memory)) || !(a->scale == a->scale)) return S2T_ERR_ARG;
   if (misaligned(a, a->k_pages, a->p_sp, a->p_sh) || misaligned(a, a->v_pages, a->p_sr, 0) || misaligned(a, a->q, a->q_st, a->q_sh) ||
       misaligned(a, a->out, a->o_st, a->o_sh) || ((uintptr_t)a->tree & 7))
     return S2T_ERR_ALIGN;

@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import kernels as K
+from . import paged
 from ._lib import require_cuda
 from .flat_params import cw, transposed
 
@@ -1896,6 +1897,34 @@ def attention_step(xq, residual, prm, H, kv, n_keys, key_lens, self_attention):
                b_s=(kv_sb, dk), c_s=(d, dk))
     y = torch.empty(Bb, d, dtype=dt, device=dev)
     K.gemm(O, cw(prm["o_w"]), y, M=Bb, N=d, K=d, lda=d, ldb=d, ldc=d, bias=prm["o_b"].data, residual=residual, ldr=d)
+    return y
+
+
+def attention_extend(xq, residual, prm, H, pages, table, lens, cu, max_new, tree=None, memory=False, keep=None):
+    """``attention_step`` for any number of new tokens of each sequence over a paged cache (s2t_amd/paged.py): ``xq`` [N, d] are the
+    (layer-normed) new tokens' rows, ``pages`` this layer's (k, v).  Self-attention appends their keys and values first (the fused QKV
+    rows go to ``keep``, a list, for a caller that will take over accepted drafts from them); with ``memory`` the pages hold the projected
+    encoder output.  Returns residual + out_proj(attention)."""
+    N, d = xq.shape
+    dk = d // H
+    dt, dev = xq.dtype, xq.device
+    if memory:
+        q = torch.empty(N, d, dtype=dt, device=dev)
+        K.gemm(xq, cw(prm["q_w"]), q, M=N, N=d, K=d, lda=d, ldb=d, ldc=d, bias=prm["q_b"].data)
+        q = q.view(N, H, dk)
+    else:
+        wqkv = fused([prm["q_w"], prm["k_w"], prm["v_w"]], 3 * d, d)
+        bqkv = fused_master([prm["q_b"], prm["k_b"], prm["v_b"]], 3 * d)
+        qkv = torch.empty(N, 3 * H, dk, dtype=dt, device=dev)
+        K.gemm(xq, wqkv, qkv, M=N, N=3 * d, K=d, lda=d, ldb=d, ldc=3 * d, bias=bqkv)
+        q = qkv[:, :H]
+        paged.paged_kv_append(qkv[:, H:2 * H], qkv[:, 2 * H:], pages[0], pages[1], table, lens, cu, max_new)
+        if keep is not None:
+            keep.append(qkv)
+    o = torch.empty(N, H, dk, dtype=dt, device=dev)
+    paged.paged_attention(q, pages[0], pages[1], table, lens, cu, max_new, tree=tree, out=o, memory=memory)
+    y = torch.empty(N, d, dtype=dt, device=dev)
+    K.gemm(o.view(N, d), cw(prm["o_w"]), y, M=N, N=d, K=d, lda=d, ldb=d, ldc=d, bias=prm["o_b"].data, residual=residual, ldr=d)
     return y
 
 

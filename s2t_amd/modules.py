@@ -523,6 +523,18 @@ class TransformerDecoderLayer(nn.Module):
         return Fn.ffn(y, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, self.activation_fn, 1.0, x,
                       0.0, 0.0, False)
 
+    def extend(self, x, state, layer, cu, max_new, tree):
+        """New tokens of many sequences at once (inference): ``x`` [N, d] their rows, ``state`` a ``PagedDecoderState``."""
+        y = self.self_attn_layer_norm(x)
+        c = state.cache
+        x = Fn.attention_extend(y, x, self.self_attn._prm(), self.self_attn.num_heads, (c.k[layer], c.v[layer]), c.table, state.lens, cu,
+                                max_new, tree=tree, keep=state.rows)
+        y = self.encoder_attn_layer_norm(x)
+        x = Fn.attention_extend(y, x, self.encoder_attn._prm(), self.encoder_attn.num_heads, state.memory[layer], state.memory_table,
+                                state.memory_lens, cu, max_new, memory=True)
+        y = self.final_layer_norm(x)
+        return Fn.ffn(y, self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias, self.activation_fn, 1.0, x, 0.0, 0.0, False)
+
     def forward(self, x, mem, B, U, Tm, self_lens, mem_lens, mem_kv=None):
         # (the LayerNorm in front of the self-attention rides in the fused q|k|v projection's prologue where the row-block
         # kernel applies, its backward in that projection's input-gradient kernel)

@@ -27,7 +27,7 @@ _I32 = torch.int32
 
 
 _NONE3 = (0, 0, 0)
-_NO_KV, _NO_APPEND, _NO_ATTENTION = (0,) * 6, (0,) * 9, (0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0)  # fields of s2t_paged_args that a call leaves out
+_NO_KV, _NO_APPEND, _NO_ATTENTION = (0,) * 6, (0,) * 9, (0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0, 0)  # fields of s2t_paged_args that a call leaves out
 
 
 def _refuse(what):
@@ -146,12 +146,14 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
     return q_out
 
 
-def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=None, scale=None, out=None, return_lse=False):
+def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=None, scale=None, out=None, return_lse=False, memory=False):
     """``softmax(scale * q k^T) v`` of the new tokens ``q [N, q_heads, head_dim]`` over their sequences' pages (the new tokens' own keys and
     values have been appended): query head h reads key/value head ``h // (q_heads // kv_heads)``.
 
     Every new token sees the whole prefix.  Of the new tokens of its sequence it sees those up to itself, or with ``tree`` (int64
     ``[N, words]``) new token j where bit ``j % 64`` of word ``j // 64`` of its row is set — its ancestors and itself, any other set will do.
+    With ``memory`` the pages hold something the new tokens only read (the projected encoder output of an encoder-decoder attention): lens
+    counts its places alone, and every new token sees all of them.
     A row that sees nothing comes out 0 with lse -inf; what a row does not see never touches it, infinities and NaN included.
     Inference only.  -> out [N, q_heads, head_dim] (``out`` if given), with ``return_lse`` also the fp32 logsumexp [N, q_heads]."""
     N, Hq, d = q.shape if q.dim() == 3 else (0, 0, 0)
@@ -159,6 +161,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
     qf = _rows("q", q, None, k_pages)
     bits = _NONE3
     if tree is not None:
+        if memory:
+            _refuse("a tree over a memory that holds no new tokens")
         if tree.dtype is not torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
             _refuse("tree must be int64 [%d, words] with contiguous rows, got %s %s" % (N, tuple(tree.shape), tree.dtype))
         bits = (tree.data_ptr(), tree.stride(0), tree.shape[1])
@@ -168,7 +172,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
     if return_lse:
         lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device)
         to_lse = lse.data_ptr()
-    tail = (to_lse, *bits, d ** -0.5 if scale is None else float(scale))
+    tail = (to_lse, *bits, d ** -0.5 if scale is None else float(scale), 1 if memory else 0)
     args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, 0, 0)
     if cache[8] * cache[9] > K.PAGED_ONE_RANGE:
         n = K.paged_attention_ws_bytes(args)
@@ -177,3 +181,43 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
             args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, ws.data_ptr(), n)
     K.paged_attention(dev, args)
     return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """Pages of ``layers`` decoder layers and the table that deals them out: a sequence takes pages as it grows (``reserve``) and gives them
+    back when it is done (``release``).  ``k[l]`` / ``v[l]`` are layer l's pages, ``table`` the tensor the functions above take; its rows
+    change on the host and reach the device with the next ``sync``."""
+
+    def __init__(self, layers, seqs, pages, pages_per_seq, kv_heads, head_dim, dtype, device, page_size=16):
+        self.page_size, self.pages_per_seq = page_size, pages_per_seq
+        self.k, self.v = (torch.empty(layers, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device) for _ in range(2))
+        self.host_table = torch.full((seqs, pages_per_seq), -1, dtype=torch.int32)
+        self.table = self.host_table.to(device, copy=True)
+        self.free = list(range(pages - 1, -1, -1))
+        self.held = [[] for _ in range(seqs)]
+        self.dirty = False
+
+    def reserve(self, seq, places):
+        """Pages for the first ``places`` places of a sequence."""
+        need = -(-places // self.page_size) - len(self.held[seq])
+        if need <= 0:
+            return
+        if need > len(self.free) or len(self.held[seq]) + need > self.pages_per_seq:
+            raise RuntimeError("paged cache: sequence %d needs %d more pages, %d are free and %d its table's row takes" % (
+                seq, need, len(self.free), self.pages_per_seq - len(self.held[seq])))
+        for _ in range(need):
+            self.host_table[seq, len(self.held[seq])] = self.free[-1]
+            self.held[seq].append(self.free.pop())
+        self.dirty = True
+
+    def release(self, seq):
+        """All pages of a sequence are free again."""
+        self.free += reversed(self.held[seq])
+        self.held[seq] = []
+        self.host_table[seq] = -1
+        self.dirty = True
+
+    def sync(self):
+        if self.dirty:
+            self.table.copy_(self.host_table)
+            self.dirty = False

@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from . import functional as Fn
 from . import kernels as K
+from . import paged
 from . import rows as Rows
 from .flat_params import FlatParameters
 from .modules import (CTC, TABLES, Adapter, Conv1dSubsampling, Ctx, LayerNorm, Linear, MaskRows,
@@ -553,6 +554,27 @@ class TransformerDecoderScriptable(nn.Module):
             x = self.layer_norm(x)
         return x.view(Bb, 1, d), {"attn": [None], "inner_states": [], "mixup": None}
 
+    def paged_state(self, encoder_out, places, page_size=16):
+        """A ``PagedDecoderState`` for the sentences of ``encoder_out``, each of at most ``places`` tokens."""
+        return PagedDecoderState(self, encoder_out, places, page_size)
+
+    def extend(self, tokens, positions, state, cu, max_new, tree=None):
+        """Pushes new tokens of many sequences through the layers in one pass: ``tokens`` [N] int64, ``positions`` [N] int32 (0 for a
+        sentence's first; in a tree of drafts the depth), rows ``cu[b] .. cu[b + 1] - 1`` of sentence b, at the end of ``state.lens[b]``
+        places; ``tree`` as s2t_amd.paged.paged_attention takes it.  -> logits [N, V].  The new tokens' keys and values are in the cache
+        afterwards, and ``state.accept`` takes over some of them in place of all."""
+        if torch.is_grad_enabled():
+            raise RuntimeError("incremental decoding is inference only: wrap the generator in torch.no_grad()")
+        tab = TABLES.get("sin", self.max_positions() + self.padding_idx + 1, self.embed_dim, tokens.device)
+        pos = positions + (self.padding_idx + 1)  # make_positions (utils.py:240-250) of tokens without padding among them
+        x = Fn.embedding(tokens, pos, self.embed_tokens.weight, tab, self.embed_scale, self.padding_idx)
+        state.rows.clear()
+        for i, layer in enumerate(self.layers):
+            x = layer.extend(x, state, i, cu, max_new, tree)
+        if self.layer_norm is not None:
+            x = self.layer_norm(x)
+        return self.output_projection(x, out_dtype=self.logits_dtype)
+
     def reorder_incremental_state(self, incremental_state, new_order):
         """modules/multihead_attention.py:574-592 / fairseq_incremental_decoder.py: caches follow the surviving beams."""
         state = incremental_state.get("s2t_amd.decoder")
@@ -581,6 +603,41 @@ class TransformerDecoderScriptable(nn.Module):
     def get_normalized_probs(self, net_output, log_probs, sample=None):
         logits = net_output[0].float()
         return torch.log_softmax(logits, dim=-1) if log_probs else torch.softmax(logits, dim=-1)
+
+
+class PagedDecoderState:
+    """What a decoder keeps between passes over a paged cache (s2t_amd/paged.py): the layers' pages, the projected encoder output of every
+    layer as pages of a memory, and the fused projections of the last pass's new tokens.  ``lens`` [B] int32 is the caller's to set before
+    each pass (places including the pass's new tokens)."""
+
+    def __init__(self, decoder, encoder_out, places, page_size):
+        mem_tbc = encoder_out["encoder_out"][0]
+        Tm, B, d = mem_tbc.shape
+        dt, dev = mem_tbc.dtype, mem_tbc.device
+        H = decoder.layers[0].self_attn.num_heads
+        n = -(-places // page_size)
+        self.cache = paged.PagedKVCache(len(decoder.layers), B, B * n, n, H, d // H, dt, dev, page_size)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=dev)
+        self.rows = []
+        # the memory: page_size frames of a sentence side by side, keys and values of a frame in one row
+        m = max(1, -(-Tm // page_size))
+        mem = torch.zeros(B, m * page_size, d, dtype=dt, device=dev)
+        mem[:, :Tm].copy_(mem_tbc.transpose(0, 1))
+        self.memory = []
+        for layer in decoder.layers:
+            he = layer.encoder_attn.num_heads
+            kv = Fn.project_memory(mem.view(-1, d), layer.encoder_attn._prm(), B * m * page_size).view(B * m, page_size, 2, he, d // he)
+            self.memory.append((kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)))
+        self.memory_table = torch.arange(B * m, dtype=torch.int32, device=dev).view(B, m)
+        self.memory_lens = (~encoder_out["encoder_padding_mask"][0]).sum(1).to(torch.int32)
+
+    def accept(self, rows, lens, cu, max_new):
+        """Of the last pass's new tokens, keeps rows ``rows`` [n] int32 (those of sentence b at ``cu[b] .. cu[b + 1] - 1``) as the last of
+        ``lens[b]`` places."""
+        c = self.cache
+        H = c.k.shape[2]
+        for layer, qkv in enumerate(self.rows):
+            paged.paged_kv_append(qkv[:, H:2 * H], qkv[:, 2 * H:], c.k[layer], c.v[layer], c.table, lens, cu, max_new, rows=rows)
 
 
 class _DictLike:
@@ -874,6 +931,10 @@ class CTCDecoder:
             # rows and emit ctc_out_dtype logits from the intermediate heads
             for mod, old in flagged:
                 mod.decode_inter_logits = old
+        return self.from_encoder(enc)
+
+    def from_encoder(self, enc):
+        """Hypotheses from an encoder dictionary that holds the decoded head's logits (or arg-max ids)."""
         has_x = len(enc.get("xctc_logit", [])) > 0
         pk = enc.get("packed")
         if pk is not None and self.ctc_inter_logit == 0 and not has_x and pk.get("ctc_greedy") is not None:

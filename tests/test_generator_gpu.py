@@ -143,3 +143,117 @@ def test_joint_ctc_beam_search_matches_oracle(golden_dir):
         for k, h in enumerate(hb):
             assert h["tokens"].tolist() == ref[b][k]["tokens"], (b, k)
             assert abs(float(h["score"]) - ref[b][k]["score"]) < 2e-3
+
+
+def _golden_generator(golden_dir, **kw):
+    z = np.load(os.path.join(golden_dir, "beam_search_transformer.npz"))
+    cfg = O.cfg_from_golden(z)
+    vocab = z["w::decoder.embed_tokens.weight"].shape[0]
+    task = M.FakeTask(vocab)
+    model = M.S2TTransformerModel.build_model(args_from_cfg(cfg, vocab), task)
+    model.load_state_dict({k[3:]: torch.from_numpy(z[k]) for k in z.files if k.startswith("w::")}, strict=True)
+    model.prepare(torch.float32, DEV)
+    sample = {"net_input": {"src_tokens": torch.from_numpy(z["in::src_tokens"]).to(DEV), "src_lengths": torch.from_numpy(z["in::src_lengths"]).to(DEV)}}
+    gen = lambda **k: SequenceGenerator([model], task.target_dictionary, max_len_a=0, max_len_b=int(z["gen::max_len_b"]), **kw, **k)  # noqa: E731
+    return gen, sample, model
+
+
+def _same_hypotheses(a, b, tol=1e-3):
+    for x, y in zip(a, b):
+        assert x[0]["tokens"].tolist() == y[0]["tokens"].tolist()
+        assert abs(float(x[0]["score"]) - float(y[0]["score"])) < tol
+        np.testing.assert_allclose(x[0]["positional_scores"].numpy(), y[0]["positional_scores"].numpy(), atol=2 * tol)
+
+
+@pytest.mark.parametrize("kw", [{}, {"min_len": 6, "unk_penalty": 0.5}, {"temperature": 1.7, "len_penalty": 0.6}, {"normalize_scores": False}])
+def test_greedy_search_with_drafts_equals_beam_one(golden_dir, kw):
+    """Whatever the drafts — the CTC head's, none, the hypotheses themselves, hypotheses with tokens replaced, dropped and put in, other
+    sentences' — the hypotheses are those of beam 1; right drafts take a fraction of the passes."""
+    gen, sample, model = _golden_generator(golden_dir, **kw)
+    want = gen(beam_size=1).generate([model], sample)
+    right = [h[0]["tokens"].tolist()[:-1] for h in want]
+    longest = max(len(h) for h in right) + 1
+    drafted = gen(beam_size=1, draft="ctc", draft_len=5)
+    _same_hypotheses(drafted.generate([model], sample), want)
+    assert drafted.draft_passes <= longest
+    edits = [[d[0] + 1] + d[1:2] + d[3:6] + [9] + d[6:] if len(d) > 6 else [7] + d for d in right]
+    for drafts in ([[] for _ in right], right, edits, [list(reversed(d)) for d in right], right[1:] + right[:1], [d + [5] * 70 for d in edits]):
+        for n in (1, 5, 40):
+            g = gen(beam_size=1, draft="ctc", draft_len=n)
+            _same_hypotheses(g.generate([model], sample, drafts=drafts), want)
+            assert g.draft_passes <= longest
+            if drafts is right and n == 40:
+                assert g.draft_passes == 1 + (longest > 41)
+
+
+def test_drafts_are_refused_where_they_cannot_verify(golden_dir):
+    gen, sample, model = _golden_generator(golden_dir)
+    with pytest.raises(ValueError, match="beam_size 1"):
+        gen(beam_size=2, draft="ctc")
+    with pytest.raises(ValueError, match="beam_size 1"):
+        gen(beam_size=1, draft="ctc", ctc_weight=0.3)
+    with pytest.raises(NotImplementedError):
+        gen(beam_size=1, draft="lm")
+    with pytest.raises(ValueError, match="drafts for"):
+        gen(beam_size=1, draft="ctc").generate([model], sample, drafts=[[5]])
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-3), (torch.bfloat16, 4e-2)])
+def test_extended_decoder_equals_teacher_forced_decoder(dtype, tol):
+    """Passes of several tokens at a time over the paged cache — ragged, some sentences bringing none, a tree of drafts whose accepted path
+    closes ranks — reproduce the positions of the full decoder (the bounds of the one-token test above)."""
+    torch.manual_seed(3)
+    V = 47
+    args = M.recipe_args(conformer=False, encoder_embed_dim=128, encoder_ffn_embed_dim=256, encoder_layers=2, decoder_layers=2,
+                         decoder_embed_dim=128, decoder_ffn_embed_dim=256, encoder_attention_heads=2, decoder_attention_heads=2,
+                         subsampling_filter=96, vocab_size=V)
+    model = M.S2TTransformerModel.build_model(args, M.FakeTask(V)).prepare(dtype, DEV)
+    model.eval()
+    g = torch.Generator().manual_seed(1)
+    B, T, U = 3, 120, 19
+    lens = torch.tensor([120, 100, 77])
+    src = torch.randn(B, T, 80, generator=g)
+    for b in range(B):
+        src[b, lens[b]:] = 0
+    prev = torch.randint(4, V, (B, U), generator=g)
+    prev[:, 0] = 2
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    with torch.no_grad():
+        enc = model.encoder(src.to(DEV), lens.to(DEV))
+        full, _ = model.decoder(prev.to(DEV), encoder_out=enc)
+        full = full.float()
+        state = model.decoder.paged_state(enc, U + 8, page_size=8)
+        for b in range(B):
+            state.cache.reserve(b, U + 8)
+        state.cache.sync()
+        done = [0] * B
+
+        def go(count, tokens, depths, tree=None):
+            cu = [0] + list(np.cumsum(count))
+            state.lens.copy_(i32([d + n for d, n in zip(done, count)]))
+            pos = [done[b] + depths[cu[b] + i] for b in range(B) for i in range(count[b])]
+            return cu, model.decoder.extend(torch.tensor(tokens, device=DEV), i32(pos), state, i32(cu), max(count), tree).float()
+
+        def near(row, b, t):
+            assert float((row - full[b, t]).abs().max() / full[b, t].abs().max()) < tol, (b, t)
+
+        for count in ([4, 1, 0], [0, 3, 7], [1, 1, 1]):
+            cu, logits = go(count, [int(prev[b, done[b] + i]) for b in range(B) for i in range(count[b])], [i for n in count for i in range(n)])
+            for b in range(B):
+                for i in range(count[b]):
+                    near(logits[cu[b] + i], b, done[b] + i)
+                done[b] += count[b]
+        # a tree: node 0 the right token, node 1 a wrong child, node 2 the right child, node 3 a wrong child of 1, node 4 the right one of 2
+        count, depths, sees = [5] * B, [0, 1, 1, 2, 2] * B, [1, 3, 5, 11, 21] * B
+        tokens = [t for b in range(B) for t in (int(prev[b, done[b]]), 6, int(prev[b, done[b] + 1]), 7, int(prev[b, done[b] + 2]))]
+        cu, logits = go(count, tokens, depths, torch.tensor(sees, device=DEV).view(-1, 1))
+        for b in range(B):
+            for node, t in ((0, 0), (2, 1), (4, 2)):
+                near(logits[cu[b] + node], b, done[b] + t)
+        done = [d + 3 for d in done]
+        state.accept(i32([cu[b] + i for b in range(B) for i in (0, 2, 4)]), i32(done), i32([0, 3, 6, 9]), 3)
+        count = [U - d for d in done]
+        cu, logits = go(count, [int(prev[b, done[b] + i]) for b in range(B) for i in range(count[b])], [i for n in count for i in range(n)])
+        for b in range(B):
+            for i in range(count[b]):
+                near(logits[cu[b] + i], b, done[b] + i)

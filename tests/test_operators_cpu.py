@@ -117,7 +117,8 @@ def test_bad_appends_are_refused(change):
 @pytest.mark.parametrize("change", [
     dict(q=torch.zeros(5, 3, 32)), dict(q=torch.zeros(5, 0, 32)), dict(q=torch.zeros(5, 4, 16)), dict(q=torch.zeros(5, 4, 32, dtype=torch.bfloat16)),
     dict(q=torch.zeros(5, 4, 64)[..., ::2]), dict(out=torch.zeros(5, 4, 16)), dict(out=torch.zeros(4, 4, 32)), dict(tree=torch.zeros(5, 1, dtype=i32)),
-    dict(tree=torch.zeros(4, 1, dtype=torch.int64)), dict(tree=torch.zeros(5, 0, dtype=torch.int64)), dict(tree=torch.zeros(2, 5, dtype=torch.int64).t())])
+    dict(tree=torch.zeros(4, 1, dtype=torch.int64)), dict(tree=torch.zeros(5, 0, dtype=torch.int64)), dict(tree=torch.zeros(2, 5, dtype=torch.int64).t()),
+    dict(tree=torch.zeros(5, 1, dtype=torch.int64), memory=True)])
 def test_bad_attention_calls_are_refused(change):
     with pytest.raises(ValueError, match="paged cache"):
         _attend(**change)
@@ -161,6 +162,7 @@ def test_the_c_entries_refuse_before_they_launch():
     assert lib.s2t_paged_kv_append(args(rows=p), None) == -1            # with q
     assert lib.s2t_paged_kv_append(args(rotary=p, rot_dim=48, rotary_positions=1), None) == -1
     assert lib.s2t_paged_attention(args(tree=p, tree_words=0), None) == -1
+    assert lib.s2t_paged_attention(args(tree=p, tree_words=1, memory=1), None) == -1
     f, b = lib.s2t_token_logprobs_fwd, lib.s2t_token_logprobs_bwd
     assert f(0, p, 8, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == 0
     assert f(0, p, 7, 0, 8, p, -1, 1.0, 0, p, p, p, None, None, None) == -1       # rows overlap
@@ -173,9 +175,76 @@ def test_the_c_entries_refuse_before_they_launch():
     assert b(0, p, 8, 1, 8, p, -1, 1.0, 2, p, None, None, None, p, None, p, 8, None) == -1  # g_top without the columns
 
 
+def test_pages_are_dealt_out_and_come_back():
+    c = paged.PagedKVCache(2, 3, 5, 4, 1, 16, torch.float32, "cpu", page_size=8)
+    c.reserve(0, 9)
+    c.reserve(1, 8)
+    c.reserve(0, 16)  # has them
+    assert c.host_table.tolist() == [[0, 1, -1, -1], [2, -1, -1, -1], [-1] * 4] and c.table.max() == -1
+    c.sync()
+    assert torch.equal(c.table, c.host_table) and not c.dirty
+    with pytest.raises(RuntimeError, match="3 more pages"):
+        c.reserve(2, 24)
+    c.release(0)
+    c.reserve(2, 24)
+    assert sorted(c.held[2]) == [0, 1, 3] and c.host_table[0].max() == -1
+    with pytest.raises(RuntimeError, match="its table's row takes"):
+        c.reserve(2, 40)
+
+
 def test_rotary_table():
     t = M.rotary_table(5, 32)
     assert t.shape == (5, 32) and torch.equal(t[0], torch.cat([torch.ones(16), torch.zeros(16)]))
     far = M.rotary_table(100001, 32)[100000].double()
     w = 10000.0 ** (-torch.arange(0, 32, 2, dtype=torch.float64) / 32)
     assert float((far - torch.cat([torch.cos(1e5 * w), torch.sin(1e5 * w)])).abs().max()) < 2.0 ** -24
+
+
+def test_drafted_sentences_say_what_the_decoder_says():
+    """The bookkeeping of greedy search with drafts against a decoder that is a table: whatever the draft, the output is the decoder's, the
+    kept nodes spell it, and a tree's words hold each node's ancestors."""
+    import random
+
+    from s2t_amd.sequence_generator import _DraftedSentence, _words
+
+    assert _words(1, 1) == [1] and _words(1 << 63, 1) == [-(1 << 63)] and _words((1 << 64) | 5, 2) == [5, 1] and _words((1 << 128) - 1, 2) == [-1, -1]
+    rng = random.Random(3)
+    for case in range(300):
+        said = [rng.randint(4, 9) for _ in range(rng.randint(0, 30))] + [2]
+        draft = list(said[:-1])
+        for _ in range(rng.randint(0, 6)):
+            i = rng.randint(0, len(draft))
+            kind = rng.random()
+            if kind < 0.4 and i < len(draft):
+                draft[i] = rng.randint(4, 9)
+            elif kind < 0.7 and i < len(draft):
+                del draft[i]
+            else:
+                draft.insert(i, rng.randint(4, 9))
+        max_len = len(said) - 1 + rng.randint(0, 3)
+        s = _DraftedSentence(draft, 2)
+        cache, passes = [], 0
+        while not s.done:
+            passes += 1
+            s.plan(rng.randint(1, 8), max_len)
+            assert max(n.depth for n in s.nodes) + s.kept <= max_len
+            before = [2] + said[:s.kept]
+            choices = []
+            for i, n in enumerate(s.nodes):
+                up = [j for j in range(len(s.nodes)) if n.sees >> j & 1]
+                assert up[-1] == i and [s.nodes[j].depth for j in up] == list(range(n.depth + 1))
+                spelt = cache + [s.nodes[j].token for j in up]
+                agrees = spelt == ([2] + said)[:len(spelt)]
+                choices.append((said[len(spelt) - 1], -0.5) if agrees else (rng.randint(4, 9), -9.0))
+            assert s.branches or all(n.sees == (2 << i) - 1 for i, n in enumerate(s.nodes))
+            path = s.walk(choices)
+            cache += [s.nodes[i].token for i in path]
+            assert cache == before + said[len(before) - 1:][:len(cache) - len(before)] and len(cache) == s.kept
+        assert s.out == said and len(s.scores) == len(said) and passes <= len(said)
+    s = _DraftedSentence(list(range(4, 24)), 2)   # a right draft of 20 tokens, 8 at a time: 9 said in the first pass, 9, then the rest
+    said, passes = list(range(4, 24)) + [2], 0
+    while not s.done:
+        s.plan(8, 40)
+        s.walk([(said[s.kept + n.depth], 0.0) for n in s.nodes])
+        passes += 1
+    assert s.out == said and passes == 3

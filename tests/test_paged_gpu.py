@@ -445,6 +445,23 @@ def test_two_runs_are_equal_on_another_stream_and_in_a_graph():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_memory_is_seen_whole_by_every_new_token(dtype):
+    """Encoder-decoder attention: lens counts the memory alone; an empty memory gives zeros; rows of 16 * 4 + 1 new tokens."""
+    c = make([3, 65, 1, 2], [40, 130, 0, 1], 4, 2, 64, 16, dtype, 71, garbage=math.nan)
+    a = on_gpu(c)
+    a["lens"] -= torch.tensor(c["news"], dtype=torch.int32, device=DEV)
+    # the exact form: the same rows, each the last new token of a sequence as long as the memory
+    full = dict(c, news=[], lens=[], cu=None)
+    for b, n in enumerate(c["news"]):
+        full["news"] += [1] * n
+        full["lens"] += [int(c["lens"][b]) - n] * n
+    full["table"] = np.concatenate([np.repeat(c["table"][b:b + 1], n, 0) for b, n in enumerate(c["news"])])
+    full["cu"] = np.arange(c["N"] + 1, dtype=np.int32)
+    full["lens"] = np.array(full["lens"])
+    check(full, paged.paged_attention(**a, memory=True, return_lse=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_calls_without_new_tokens(dtype):
     c = make([0, 0], [5, 0], 2, 1, 32, 16, dtype, 61)
     a = on_gpu(c)
