@@ -555,7 +555,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
     if (row >= rc.rows || col >= d) continue;
     const int i = tok[mt], t = sp.row0 + i, hq = h * group + row - i * group;
     if (used == 1) {
-      const float inv = top == -INFINITY ? 0.f : 1.f / total;
+      const float inv = total == 0.f ? 0.f : 1.f / total;  // (nothing seen; a NaN score leaves a sum of NaN, and so does its row)
       T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
 #pragma unroll
       for (int dt = 0; dt < NDT; dt += 2) {
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
           out[dt + 1] = o[dt + 1] * inv;
         }
       }
-      if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
+      if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
     } else {  // part: [split][token][query head][d], then their [2]: reference and sum
       const int64_t heads = (int64_t)a.N * a.q_heads, at = split * heads + (int64_t)t * a.q_heads + hq;
       float* to = part + at * d + col;
@@ -627,12 +627,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[r] = (sums[0][col + r] + sums[1][col + r]) + (sums[2][col + r] + sums[3][col + r]);
   }
-  const float inv = top == -INFINITY ? 0.f : 1.f / total;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
   if (lane < lanes && col < d) {
     const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     st4_from_f32<T>((T*)a.out + t * a.o_st + hq * a.o_sh + col, y);
   }
-  if (a.lse && lane == 0) a.lse[at] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * LN2;
+  if (a.lse && lane == 0) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
 }
 
 // How a call is cut: rows of a tile, tiles of a sequence, ranges of the keys.
@@ -694,7 +694,7 @@ int paged_args_bad(const s2t_paged_args* a) {
   if (a->dtype != S2T_F32 && a->dtype != S2T_BF16) return S2T_ERR_DTYPE;
   if (a->B <= 0 || a->B > 65535 || a->N < 0 || a->max_new < 0 || a->q_heads <= 0 || a->kv_heads <= 0 || a->q_heads % a->kv_heads) return S2T_ERR_ARG;
   if (a->num_pages <= 0 || a->table_pages <= 0 || a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return S2T_ERR_ARG;
-  if ((int64_t)a->table_pages * a->page_size > 0x7fffff00ll) return S2T_ERR_UNSUPPORTED;  // places are 32-bit numbers
+  if ((int64_t)a->table_pages * a->page_size > 0x7fff0000ll) return S2T_ERR_UNSUPPORTED;  // places are 32-bit numbers
   if (a->dk <= 0 || a->dk % 16 || a->dk > 256) return S2T_ERR_UNSUPPORTED;
   return S2T_OK;
 }

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
     for (int e = 0; e < N; ++e) {
       const float d = fmaf(x[e], c2, -ref), p = exp2_(d);
       st.s += p;
-      if (ENTROPY) st.t = fmaf(p, fmaxf(d, -1e30f), st.t);  // (a column of -inf: 0 * -1e30)
+      if (ENTROPY) st.t = fmaf(p, fmaxf(d, -1e3f), st.t);  // (a column of -inf: 0 * -1e3)
     }
   };
   for (int v0 = tid; v0 < nvec; v0 += THREADS * NB) {
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
   // (a column of -inf: p is 0, and so is its gradient)
   auto dense = [&](float x) {
     const float lp = fmaf(x, c2, -L2);
-    return -exp2_(lp) * fmaf(gp, fmaxf(lp, -1e30f), gw);
+    return -exp2_(lp) * fmaf(gp, fmaxf(lp, -1e3f), gw);
   };
   for (int v0 = tid; v0 < nvec; v0 += 256 * NB) {
     Vec buf[NB];

@@ -194,6 +194,8 @@ class SequenceGenerator:
         assert self.min_len <= max_len, "min_len cannot be larger than max_len, please adjust these!"
         enc = model.encoder(src_tokens, net_input["src_lengths"])
         if drafts is None:
+            if not any(len(enc.get(k, [])) for k in ("ctc_logit", "xctc_logit")):
+                raise ValueError("the model has no CTC head to draft with: pass drafts")
             drafts = [h[0]["tokens"].tolist() for h in CTCDecoder([model], dictionary=self.tgt_dict, blank_idx=self.blank).from_encoder(enc)]
         if len(drafts) != bsz:
             raise ValueError("%d drafts for %d sentences" % (len(drafts), bsz))

@@ -213,6 +213,24 @@ def test_infinite_values_that_are_seen(dtype):
             assert inf == [[1, 5]] and nan == []
 
 
+@pytest.mark.parametrize("splits", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_scores_that_are_seen(dtype, splits):
+    """A NaN in a key makes the rows that see it NaN (those that see nothing else too), and no other row; so does one in a query."""
+    c = make([6, 1, 2], [20 if not splits else 3000, 0, 40], 2, 2, 64, 16, dtype, 12)
+    sees, words = random_tree(c)
+    place = int(c["lens"][0]) - 6 + 3                                              # new token 3 of sequence 0, head 1
+    c["k"][c["table"][0, place // 16], 1, place % 16, 5] = math.nan
+    c["k"][c["table"][1, 0], 0, 0, 0] = math.nan                                   # all that sequence 1's only token sees in head 0
+    c["q"][8, 1, 2] = math.nan
+    out, lse = (x.cpu().float() for x in paged.paged_attention(**on_gpu(c), tree=words.to(DEV), return_lse=True))
+    want = torch.zeros(9, 2, dtype=torch.bool)
+    want[:6, 1] = torch.from_numpy(sees[:6, 3])
+    want[6, 0] = want[8, 1] = True
+    assert torch.equal(lse.isnan(), want) and torch.equal(out.isnan(), want[..., None].expand(9, 2, 64))
+    assert out[~want].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_large_scores_and_a_scale_of_ones_own(dtype):
     """Scores of several hundred: the running maximum has to carry the sum; a negative and a zero scale are scales too."""

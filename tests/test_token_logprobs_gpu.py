@@ -211,6 +211,42 @@ def test_an_empty_batch_and_partial_gradients():
         assert float((dx.cpu().double() - grad).abs().max()) <= 40 * _ep(x.cpu(), 1.0)  # |upstream| <= 4 in four terms, H <= log 77 < 5
 
 
+def test_gradients_of_broadcast_logits_and_of_a_tensor_used_twice():
+    """One row expanded to five, and the same logits scored for two sets of tokens: the gradients add up."""
+    x, g = _logits(1, 50, torch.float32, 6, pad=False)
+    tokens = torch.randint(0, 50, (5,), generator=g)
+    up = torch.randn(5, generator=g)
+    leaf = x.detach().requires_grad_()
+    a = Fn.token_logprobs(leaf.expand(5, 50), tokens.to(DEV)).logprob
+    b = Fn.token_logprobs(leaf, tokens[:1].to(DEV), entropy=True)
+    (dx,) = torch.autograd.grad([a, b.logprob, b.entropy], leaf, [up.to(DEV), torch.ones(1, device=DEV), torch.ones(1, device=DEV)])
+    xc = x.double().cpu().requires_grad_()
+    lp = torch.log_softmax(xc, -1)
+    (lp.expand(5, 50).gather(1, tokens[:, None])[:, 0] * up.double()).sum().add(lp[0, tokens[0]] - (lp.exp() * lp).sum()).backward()
+    assert float((dx.cpu().double() - xc.grad).abs().max()) <= 60 * _ep(x.cpu(), 1.0)  # seven terms, |upstream| <= 3, H <= log 50 < 4
+
+
+def test_logits_beyond_32_bit_offsets():
+    """66 000 rows of 33 000: 2.2e9 elements; every row of zeros scores -log V, the last ones their own values, the gradient reaches them."""
+    rows, V = 66000, 33000
+    x = torch.zeros(rows, V, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    x[-2:] = torch.randn(2, V, generator=g).bfloat16().to(DEV)
+    tokens = torch.arange(rows, device=DEV) % V
+    leaf = x.requires_grad_()
+    r = Fn.token_logprobs(leaf, tokens, top=2)
+    assert float((r.logprob[:-2] + math.log(V)).abs().max()) <= E * (V / 64 + 64)
+    want = torch.log_softmax(x[-2:].detach().double().cpu(), -1)
+    at = tokens[-2:].cpu()
+    assert float((r.logprob[-2:].detach().cpu().double() - want.gather(1, at[:, None])[:, 0]).abs().max()) <= _ep(x[-2:].detach().float().cpu(), 1.0)
+    assert torch.equal(r.top_index[-2:].cpu(), torch.sort(x[-2:].detach().float().cpu(), dim=-1, descending=True, stable=True).indices[:, :2])
+    (dx,) = torch.autograd.grad(r.logprob[-1], leaf)
+    assert not dx[:-1].any()
+    exact = -want[1].exp()
+    exact[at[1]] += 1
+    assert bool(((dx[-1].cpu().double() - exact).abs() <= 2.0 ** -8 * exact.abs() + _ep(x[-1:].detach().float().cpu(), 1.0) * 2).all())
+
+
 def test_a_second_derivative_is_refused():
     x, g = _logits(2, 9, torch.float32, 1)
     leaf = x.detach().requires_grad_()
