@@ -162,7 +162,8 @@ __device__ __forceinline__ uint32_t tree_window(const int64_t* __restrict__ row,
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // T: type of the cache; DK: head_dim rounded up to 32, 64, 128 or 256; BIG: a half tile of 16 keys lies in one page
-template <typename T, int DK, int MT, bool BIG>
+// BYROWS: the four waves have 16 * MT rows each and go over all keys (n_split is 1)
+template <typename T, int DK, int MT, bool BIG, bool BYROWS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int n_tiles, const int n_split,
                                                               const float c2, const int flip, float* __restrict__ part) {
   constexpr bool BF = sizeof(T) == 2;
@@ -170,6 +171,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   constexpr int KE = BF ? 8 : 4;        // elements of 16 bytes
   constexpr int NK = DK / (4 * KE);     // 16-byte loads of a key
   constexpr int VB = NDT * (int)sizeof(T);  // bytes that a lane loads of a value row
+  constexpr int STEP = BYROWS ? 32 : 128;   // from a tile of a wave to its next
   __shared__ float obuf[4][MT][4][64][NDT];
   __shared__ float mlbuf[4][MT][16][2];
 
@@ -186,17 +188,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   }
   if (pair >= pairs || unit >= per) return;
   const int b = pair / a.kv_heads, h = pair % a.kv_heads;
-  const int split = unit % n_split, row_base = (n_tiles - 1 - unit / n_split) * 16 * MT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = BYROWS ? 0 : unit % n_split, tile = n_tiles - 1 - (BYROWS ? unit : unit / n_split);
+  const int row_base = (BYROWS ? tile * 4 + wave : tile) * 16 * MT;
   const int group = a.q_heads / a.kv_heads;
   const Span sp = span_of(a, b);
   const Reach rc = reach_of(a, sp, shift, group, row_base, 16 * MT);
   if (row_base >= rc.rows) return;
-  const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
+  const int chunk = BYROWS ? 0 : chunk_of(rc.kend, n_split), used = BYROWS ? 1 : ranges_of(rc.kend, chunk);
   if (split >= used) return;
-  const int k_hi = min(rc.kend, (split + 1) * chunk);
+  const int k_hi = BYROWS ? rc.kend : min(rc.kend, (split + 1) * chunk);
   const int all_see = rc.prefix + (a.tree ? 0 : row_base / group + 1);  // every row of the tile sees the keys before this one
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int d = a.dk;
   const T* kpool = (const T*)a.k_pages + h * a.p_sh;
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
       for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     u32x4 kf[2][NK];
-    int key0 = split * chunk + 32 * wave;
+    int key0 = BYROWS ? 0 : split * chunk + 32 * wave;
     Where w;
     uint32_t vr[8][VW];
     Pair e{0, 0};
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
       w = find(key0, entries(key0));
       load_k(w, kf);
       load_v(w, vr);
-      e = entries(key0 + 128);
+      e = entries(key0 + STEP);
     }
     // A tile's keys and values are both on their way while the tile before it is worked on.  (The last tile asks for itself once more
     // instead of for nothing: behind a branch the compiler would have every wait for keys wait for the values as well.)
@@ -352,12 +355,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
           s[mt][t] = x;
         }
       const Where now = w;
-      const int next = key0 + 128;
+      const int next = key0 + STEP;
       if constexpr (careful) load_v(now, vr);
       else {
         if (next < k_hi) w = find(next, e);
         load_k(w, kf);
-        e = entries(next + 128);
+        e = entries(next + STEP);
       }
       __builtin_amdgcn_sched_barrier(0);
       // keys of this tile that exist, and whether every row sees all of them
@@ -517,10 +520,48 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
       for (int r = 0; r < 4; ++r) sick = fmaf(acc[mt][dt][r], 0.f, sick);
   if (__any(sick != sick)) go(std::true_type{});
 
-  // the four waves' results; wave w then finishes rows 4g + w of every 16 columns
+  // columns (4g + r) * NDT .. of query c of row tile mt: o / total, or both for paged_combine_kernel
+  auto finish = [&](int mt, int r, const float (&o)[NDT], float top, float total) {
+    const int row = row_base + mt * 16 + c, col = (4 * g + r) * NDT;
+    if (row >= rc.rows || col >= d) return;
+    const int i = tok[mt], t = sp.row0 + i, hq = h * group + row - i * group;
+    if (used == 1) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;  // (nothing seen; a NaN score leaves a sum of NaN, and so does its row)
+      T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt += 2) {
+        if constexpr (BF) *reinterpret_cast<uint32_t*>(out + dt) = bf16pack(o[dt] * inv, o[dt + 1] * inv);
+        else {
+          out[dt] = o[dt] * inv;
+          out[dt + 1] = o[dt + 1] * inv;
+        }
+      }
+      if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
+    } else {  // part: [split][token][query head][d], then their [2]: reference and sum
+      const int64_t heads = (int64_t)a.N * a.q_heads, at = split * heads + (int64_t)t * a.q_heads + hq;
+      float* to = part + at * d + col;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt += 2) *reinterpret_cast<float2*>(to + dt) = make_float2(o[dt], o[dt + 1]);
+      if (col == 0) reinterpret_cast<float2*>(part + n_split * heads * d)[at] = make_float2(top, total);
+    }
+  };
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) l[mt] = s2t_xadd<16>(s2t_xadd<32>(l[mt]));
+  if constexpr (BYROWS) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float o[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] = acc[mt][dt][r];
+        finish(mt, r, o, m[mt], l[mt]);
+      }
+    return;
+  }
+  // the four waves' results meet; wave w then finishes rows 4g + w of every 16 columns
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    l[mt] = s2t_xadd<16>(s2t_xadd<32>(l[mt]));
     if (g == 0) {
       mlbuf[wave][mt][c][0] = m[mt];
       mlbuf[wave][mt][c][1] = l[mt];
@@ -551,28 +592,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[dt] += f * obuf[w][mt][wave][lane][dt];
     }
-    const int row = row_base + mt * 16 + c, col = (4 * g + wave) * NDT;
-    if (row >= rc.rows || col >= d) continue;
-    const int i = tok[mt], t = sp.row0 + i, hq = h * group + row - i * group;
-    if (used == 1) {
-      const float inv = total == 0.f ? 0.f : 1.f / total;  // (nothing seen; a NaN score leaves a sum of NaN, and so does its row)
-      T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
-#pragma unroll
-      for (int dt = 0; dt < NDT; dt += 2) {
-        if constexpr (BF) *reinterpret_cast<uint32_t*>(out + dt) = bf16pack(o[dt] * inv, o[dt + 1] * inv);
-        else {
-          out[dt] = o[dt] * inv;
-          out[dt + 1] = o[dt + 1] * inv;
-        }
-      }
-      if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
-    } else {  // part: [split][token][query head][d], then their [2]: reference and sum
-      const int64_t heads = (int64_t)a.N * a.q_heads, at = split * heads + (int64_t)t * a.q_heads + hq;
-      float* to = part + at * d + col;
-#pragma unroll
-      for (int dt = 0; dt < NDT; dt += 2) *reinterpret_cast<float2*>(to + dt) = make_float2(o[dt], o[dt + 1]);
-      if (col == 0) reinterpret_cast<float2*>(part + n_split * heads * d)[at] = make_float2(top, total);
-    }
+    finish(mt, wave, o, top, total);
   }
 }
 
@@ -635,18 +655,32 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args
   if (a.lse && lane == 0) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
 }
 
-// How a call is cut: rows of a tile, tiles of a sequence, ranges of the keys.
+// How a call is cut: row tiles of 16 rows to a wave, whether the waves of a workgroup have rows of their own, tiles of a sequence, ranges of
+// the keys.
 struct Cut {
-  int mt, tiles, splits;
+  int mt, by_rows, tiles, splits;
 };
 Cut cut_of(const s2t_paged_args* a) {
-  const int64_t rows = (int64_t)a->max_new * (a->q_heads / a->kv_heads);
-  const int most = a->dk <= 64 ? 4 : a->dk <= 128 ? 2 : 1;
+  const int64_t rows = (int64_t)a->max_new * (a->q_heads / a->kv_heads), keys = (int64_t)a->table_pages * a->page_size;
+  const int64_t pairs = (int64_t)a->kv_heads * a->B;
   Cut c;
+  // Few keys and many rows: a wave's rows go over all keys, and nothing has to be put together (147 sequences x 8 heads x 160 rows over 76
+  // keys, fp32 heads of 64: 137 us by keys, 55 by rows; 105 x 4 x 51 over 263, bf16 heads of 128: 31.6 and 19.0), where that gives every
+  // compute unit a workgroup (2 x 8 x 164 over 288: 11.5 by keys, 15.2 by rows).
+  c.by_rows = rows > 16 && keys <= 512 && (rows + 63) / 64 * pairs >= 256;
+  if (c.by_rows) {
+    c.mt = c.splits = 1;
+    c.tiles = (int)((rows + 63) / 64);
+    return c;
+  }
+  // as many rows to a wave as registers allow, unless that leaves most of the chip without work also with the keys in ranges (568 rows of
+  // one fp32 head of 128, four sequences: 19.1 us with 32 rows, 13.6 with 16; 1248 rows of 8 heads of 32 over 2600 keys: 26.3 with 64,
+  // 22.6 with 32; but 20 rows of 4 heads of 128 over 131 000 keys: 56 with 32, 81 with 16, which reads the keys twice)
+  const int most = a->dk <= 64 ? 4 : a->dk <= 128 ? 2 : 1;
   c.mt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  while (c.mt > 1 && (rows + 16 * c.mt - 1) / (16 * c.mt) * pairs * std::max<int64_t>(1, keys / 2048) < 256) c.mt /= 2;
   c.tiles = (int)((rows + 16 * c.mt - 1) / (16 * c.mt));
-  const int64_t units = (int64_t)c.tiles * a->kv_heads * a->B, keys = (int64_t)a->table_pages * a->page_size;
-  int64_t s = (c.mt * a->dk > 128 ? 256 : 512) / units;
+  int64_t s = (c.mt * a->dk > 128 ? 256 : 512) / (c.tiles * pairs);
   if (s > keys / MIN_CHUNK) s = keys / MIN_CHUNK;
   if (s > 256) s = 256;
   if (s < 1) s = 1;
@@ -654,18 +688,23 @@ Cut cut_of(const s2t_paged_args* a) {
   return c;
 }
 
-template <typename T, int DK, int MT>
+template <typename T, int DK, int MT, bool BYROWS = false>
 void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
   const int64_t pairs = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8;
   const dim3 grid((unsigned)(pairs * c.tiles * c.splits));
   const int shift = __builtin_ctz((unsigned)a->page_size), flip = a->scale < 0.f;
   const float c2 = fmaxf(fabsf(a->scale) * LOG2E, 1e-30f);  // never 0: 0 times the -inf of a hidden key is not 0
-  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true, BYROWS>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false, BYROWS>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
 }
 template <typename T>
 void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
-  if (a->dk <= 32) {
+  if (c.by_rows) {
+    if (a->dk <= 32) launch_attention<T, 32, 1, true>(a, c, st);
+    else if (a->dk <= 64) launch_attention<T, 64, 1, true>(a, c, st);
+    else if (a->dk <= 128) launch_attention<T, 128, 1, true>(a, c, st);
+    else launch_attention<T, 256, 1, true>(a, c, st);
+  } else if (a->dk <= 32) {
     if (c.mt == 1) launch_attention<T, 32, 1>(a, c, st);
     else if (c.mt == 2) launch_attention<T, 32, 2>(a, c, st);
     else launch_attention<T, 32, 4>(a, c, st);

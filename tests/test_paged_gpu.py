@@ -141,6 +141,9 @@ SHAPES = [
     ([7, 20], [90, 3], 2, 1, 256, 4),
     ([2], [5000], 16, 2, 64, 128),
     ([257], [300], 2, 2, 112, 2),
+    ([17, 30, 1, 0] * 16, [0, 90, 40, 7] * 16, 8, 4, 64, 16),      # few keys, many rows: waves with rows of their own
+    ([5, 40] * 24, [100, 3] * 24, 12, 6, 32, 4),
+    ([23] * 66, [9] * 66, 4, 4, 128, 32),
 ]
 
 
