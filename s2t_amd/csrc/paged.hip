@@ -135,9 +135,10 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 
 // keys of each of n_split ranges of a row tile that sees keys 0 .. kend - 1
 __device__ __forceinline__ int chunk_of(int kend, int n_split) {
-  return max(MIN_CHUNK, ((kend + n_split - 1) / n_split + 127) & ~127);
+  return n_split == 1 ? max(MIN_CHUNK, kend) : max(MIN_CHUNK, ((kend + n_split - 1) / n_split + 127) & ~127);
 }
-__device__ __forceinline__ int ranges_of(int kend, int chunk) { return max(1, (kend + chunk - 1) / chunk); }
+__device__ __forceinline__ int ranges_of(int kend, int chunk) { return kend <= chunk ? 1 : (kend + chunk - 1) / chunk; }
+__device__ __forceinline__ int over(int n, int group) { return group == 1 ? n : n / group; }  // (a division is some thirty instructions)
 
 // what a row tile sees: rows of this launch, first key after the last that any of its rows may see
 struct Reach {
@@ -148,7 +149,7 @@ __device__ __forceinline__ Reach reach_of(const s2t_paged_args& a, const Span& s
   r.rows = min(s.n, a.max_new) * group;
   r.len = min(s.len, a.table_pages << shift);
   r.prefix = a.memory ? r.len : s.len - s.n;
-  const int last = (min(row_base + tile_rows, r.rows) - 1) / group;
+  const int last = over(min(row_base + tile_rows, r.rows) - 1, group);
   r.kend = a.tree ? r.len : min(r.len, r.prefix + last + 1);
   return r;
 }
@@ -164,8 +165,9 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // T: type of the cache; DK: head_dim rounded up to 32, 64, 128 or 256; BIG: a half tile of 16 keys lies in one page
 // BYROWS: the four waves have 16 * MT rows each and go over all keys (n_split is 1)
 template <typename T, int DK, int MT, bool BIG, bool BYROWS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int n_tiles, const int n_split,
-                                                              const float c2, const int flip, float* __restrict__ part) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int group, const int spread,
+                                                              const int n_tiles, const int n_split, const float c2, const int flip,
+                                                              float* __restrict__ part) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = DK / 16;          // 16-column tiles of the output
   constexpr int KE = BF ? 8 : 4;        // elements of 16 bytes
@@ -175,30 +177,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   __shared__ float obuf[4][MT][4][64][NDT];
   __shared__ float mlbuf[4][MT][16][2];
 
-  // all row tiles of a (sequence, key/value head) on one XCD (workgroups go round the eight), the longest tiles first
-  const int per = n_tiles * n_split, pairs = a.B * a.kv_heads;
-  int pair, unit;
-  if (n_tiles > 1 && pairs >= 8) {
-    const int slot = blockIdx.x >> 3;
-    pair = (slot / per) * 8 + (blockIdx.x & 7);
-    unit = slot % per;
-  } else {
-    pair = blockIdx.x % pairs;
-    unit = blockIdx.x / pairs;
-  }
-  if (pair >= pairs || unit >= per) return;
-  const int b = pair / a.kv_heads, h = pair % a.kv_heads;
+  // SPREAD: grid (8 * units, pairs / 8): all row tiles and ranges of a (sequence, key/value head) on one XCD (workgroups go round the eight),
+  // the longest tiles first; otherwise (pairs, units)
+  const int pair = spread ? blockIdx.y * 8 + (blockIdx.x & 7) : blockIdx.x, unit = spread ? blockIdx.x >> 3 : blockIdx.y;
+  if (pair >= a.B * a.kv_heads) return;
+  const int b = a.kv_heads == 1 ? pair : pair / a.kv_heads, h = pair - b * a.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = BYROWS ? 0 : unit % n_split, tile = n_tiles - 1 - (BYROWS ? unit : unit / n_split);
+  const int slow = BYROWS || n_split == 1 ? unit : unit / n_split;
+  const int split = unit - slow * n_split, tile = n_tiles - 1 - slow;
   const int row_base = (BYROWS ? tile * 4 + wave : tile) * 16 * MT;
-  const int group = a.q_heads / a.kv_heads;
   const Span sp = span_of(a, b);
   const Reach rc = reach_of(a, sp, shift, group, row_base, 16 * MT);
   if (row_base >= rc.rows) return;
   const int chunk = BYROWS ? 0 : chunk_of(rc.kend, n_split), used = BYROWS ? 1 : ranges_of(rc.kend, chunk);
   if (split >= used) return;
   const int k_hi = BYROWS ? rc.kend : min(rc.kend, (split + 1) * chunk);
-  const int all_see = rc.prefix + (a.tree ? 0 : row_base / group + 1);  // every row of the tile sees the keys before this one
+  const int all_see = rc.prefix + (a.tree ? 0 : over(row_base, group) + 1);  // every row of the tile sees the keys before this one
 
   const int c = lane & 15, g = lane >> 4;
   const int d = a.dk;
@@ -214,7 +208,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   for (int mt = 0; mt < MT; ++mt) {
     const int row = row_base + mt * 16 + c;
     const bool live = row < rc.rows;
-    tok[mt] = !live ? 0 : group == 1 ? row : row / group;
+    tok[mt] = !live ? 0 : over(row, group);
     const T* q = (const T*)a.q + (int64_t)(sp.row0 + tok[mt]) * a.q_st + (int64_t)(h * group + (live ? row - tok[mt] * group : 0)) * a.q_sh;
 #pragma unroll
     for (int ks = 0; ks < NK; ++ks) {
@@ -690,12 +684,12 @@ Cut cut_of(const s2t_paged_args* a) {
 
 template <typename T, int DK, int MT, bool BYROWS = false>
 void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
-  const int64_t pairs = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8;
-  const dim3 grid((unsigned)(pairs * c.tiles * c.splits));
-  const int shift = __builtin_ctz((unsigned)a->page_size), flip = a->scale < 0.f;
+  const int pairs = a->B * a->kv_heads, units = c.tiles * c.splits, spread = c.tiles > 1 && pairs >= 8;
+  const dim3 grid = spread ? dim3(8u * units, (unsigned)((pairs + 7) / 8)) : dim3((unsigned)pairs, (unsigned)units);
+  const int shift = __builtin_ctz((unsigned)a->page_size), flip = a->scale < 0.f, group = a->q_heads / a->kv_heads;
   const float c2 = fmaxf(fabsf(a->scale) * LOG2E, 1e-30f);  // never 0: 0 times the -inf of a hidden key is not 0
-  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true, BYROWS>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false, BYROWS>), grid, dim3(256), 0, st, *a, shift, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c2, flip, (float*)a->ws);
 }
 template <typename T>
 void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
@@ -780,9 +774,11 @@ extern "C" int s2t_paged_attention(const s2t_paged_args* a, void* stream) {
   if (a->N == 0 || a->max_new == 0) return S2T_OK;
   if (!a->q || !a->out) return S2T_ERR_ARG;
   const Cut c = cut_of(a);
-  const int64_t blocks = ((int64_t)a->B * a->kv_heads + 7) / 8 * 8 * c.tiles * c.splits;
-  // launch bounds, and 32-bit offsets of the 16 rows of a half tile
-  if (blocks > 0x7fffffff || (int64_t)a->max_new * a->q_heads > 0x7ffffff0 || a->p_sr < 0 || a->p_sr > (1 << 24)) return S2T_ERR_UNSUPPORTED;
+  // launch bounds (a grid's second dimension is 16 bits), and 32-bit offsets of the 16 rows of a half tile
+  const int64_t pairs = (int64_t)a->B * a->kv_heads, units = (int64_t)c.tiles * c.splits;
+  const bool spread = c.tiles > 1 && pairs >= 8;
+  if ((spread ? (pairs + 7) / 8 : units) > 65535 || (spread ? 8 * units : pairs) > (1 << 23) || (int64_t)a->max_new * a->q_heads > (1 << 23) || a->p_sr < 0 || a->p_sr > (1 << 24))
+    return S2T_ERR_UNSUPPORTED;
   if (c.splits > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < s2t_paged_attention_ws_bytes(a))) return S2T_ERR_ARG;
   if (a->dtype == S2T_F32) launch_attention<float>(a, c, (hipStream_t)stream);
   else launch_attention<bf16_t>(a, c, (hipStream_t)stream);
