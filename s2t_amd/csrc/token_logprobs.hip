@@ -1,5 +1,7 @@
 // Scores of given tokens over a row of logits (log probability, entropy, best alternatives) and their gradient.
 // Semantics: include/s2t_hip.h, s2t_token_logprobs_fwd / _bwd.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -45,7 +47,7 @@ struct Best {
 __device__ __forceinline__ bool before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
 
 // One workgroup to a row, one pass: every thread keeps the statistics of its vectors (relative to its own running maximum, moved once
-// for each NB vectors) and, for the alternatives, the maximum of its raw logits.  The top-th largest of the 64 maxima of four threads
+// for each NB vectors) and, for the alternatives, the maximum of its raw logits.  The top-th largest of the 64 maxima of every 64th thread
 // each bounds the alternatives from below, since as many columns reach it; the columns of the threads that reach it are read once more
 // (from the caches, dealt to all threads), those that reach it, usually hardly more than `top`, are collected and ranked by (logit, column).  Rows with more than
 // CAND such columns (ties without end) are ranked one column after the other instead.
@@ -217,8 +219,8 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
 
 // d logits of one row: -p (W + g_entropy (log p + H)) / T with W = g_logprob + sum g_top; the thread that stored the column of the token or of
 // an alternative stores it once more with its own gradient added before the rounding.
-template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V,
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V,
                                                                  const int64_t* __restrict__ tokens, int64_t ignore, float inv_temp, int top,
                                                                  const float* __restrict__ lse, const float* __restrict__ entropy,
                                                                  const float* __restrict__ g_lp, const float* __restrict__ g_ent,
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
   const int nvec = V / E, tail = nvec * E + tid;
   const int64_t y = tokens ? tokens[r] : -1;
   if (tokens && y == ignore) {
-    for (int v = tid; v < nvec; v += 256) *reinterpret_cast<Vec*>(out + (int64_t)v * E) = Vec{{0, 0, 0, 0}};
+    for (int v = tid; v < nvec; v += THREADS) *reinterpret_cast<Vec*>(out + (int64_t)v * E) = Vec{{0, 0, 0, 0}};
     if (tail < V) st_from_f32<T>(out + tail, 0.f);
     return;
   }
@@ -248,13 +250,13 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
     const float lp = fmaf(x, c2, -L2);
     return -exp2_(lp) * fmaf(gp, fmaxf(lp, -1e3f), gw);
   };
-  for (int v0 = tid; v0 < nvec; v0 += 256 * NB) {
+  for (int v0 = tid; v0 < nvec; v0 += THREADS * NB) {
     Vec buf[NB];
 #pragma unroll
-    for (int u = 0; u < NB; ++u) buf[u] = *reinterpret_cast<const Vec*>(row + (int64_t)min(v0 + u * 256, nvec - 1) * E);
+    for (int u = 0; u < NB; ++u) buf[u] = *reinterpret_cast<const Vec*>(row + (int64_t)min(v0 + u * THREADS, nvec - 1) * E);
 #pragma unroll
     for (int u = 0; u < NB; ++u)
-      if (v0 + u * 256 < nvec) {
+      if (v0 + u * THREADS < nvec) {
         float x[E];
         unpack<T>(buf[u], x);
         Vec o;
@@ -263,14 +265,14 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
           if constexpr (sizeof(T) == 2) o.w[q] = bf16pack(inv_temp * dense(x[2 * q]), inv_temp * dense(x[2 * q + 1]));
           else o.w[q] = __float_as_uint(inv_temp * dense(x[q]));
         }
-        *reinterpret_cast<Vec*>(out + (int64_t)(v0 + u * 256) * E) = o;
+        *reinterpret_cast<Vec*>(out + (int64_t)(v0 + u * THREADS) * E) = o;
       }
   }
   if (tail < V) st_from_f32<T>(out + tail, inv_temp * dense(ld_as_f32<T>(row + tail)));
   for (int k = 0; k <= (g_top ? top : 0); ++k) {
     const int64_t c = k == 0 ? y : top_idx[r * top + k - 1];
     if ((uint64_t)c >= (uint64_t)V || (k == 0 && !g_lp)) continue;
-    if (tid != (c < (int64_t)nvec * E ? (int)(c / E % 256) : (int)(c - (int64_t)nvec * E))) continue;
+    if (tid != (c < (int64_t)nvec * E ? (int)(c / E % THREADS) : (int)(c - (int64_t)nvec * E))) continue;
     float add = c == y ? gl : 0.f;
     if (g_top)
       for (int q = 0; q < top; ++q)
@@ -279,19 +281,41 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(const T* __rest
   }
 }
 
-template <typename T, int THREADS>
+// Threads of a row: five vectors each take all of a row of up to 5, 10 and 20 KB at once, and short rows leave room for many workgroups on a
+// compute unit (8000 x 2500 bf16 with 10 alternatives: 36 us with 256 threads, 18 with 64; 8000 x 5000: 36 and, with 128, 24; 2047 x 32001
+// fp32: 53 with 256, 50 with 512; 8192 x 10000 bf16: 28 with 256, 46 with 512).
+template <typename F>
+void for_threads(int64_t row_bytes, F&& f) {
+  if (row_bytes <= 5120) f(std::integral_constant<int, 64>{});
+  else if (row_bytes <= 10240) f(std::integral_constant<int, 128>{});
+  else if (row_bytes <= 65536) f(std::integral_constant<int, 256>{});
+  else f(std::integral_constant<int, 512>{});
+}
+
+template <typename T>
 void launch_fwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, float* logprob,
                 float* lse, float* entropy, float* top_lp, int64_t* top_idx, hipStream_t s) {
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, logprob, lse, entropy, top_lp, top_idx);
-  };
-  if (top > 0) {
-    if (entropy) go(token_logprobs_kernel<T, THREADS, true, true>);
-    else go(token_logprobs_kernel<T, THREADS, true, false>);
-  } else {
-    if (entropy) go(token_logprobs_kernel<T, THREADS, false, true>);
-    else go(token_logprobs_kernel<T, THREADS, false, false>);
-  }
+  for_threads((int64_t)V * sizeof(T), [&](auto n) {
+    constexpr int THREADS = decltype(n)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, logprob, lse, entropy, top_lp, top_idx);
+    };
+    if (top > 0) {
+      if (entropy) go(token_logprobs_kernel<T, THREADS, true, true>);
+      else go(token_logprobs_kernel<T, THREADS, true, false>);
+    } else {
+      if (entropy) go(token_logprobs_kernel<T, THREADS, false, true>);
+      else go(token_logprobs_kernel<T, THREADS, false, false>);
+    }
+  });
+}
+template <typename T>
+void launch_bwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, const float* lse,
+                const float* entropy, const float* g_lp, const float* g_ent, const float* g_top, const int64_t* top_idx, void* dlogits, int64_t ldd, hipStream_t s) {
+  for_threads((int64_t)V * sizeof(T), [&](auto n) {
+    constexpr int THREADS = decltype(n)::value;
+    hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, THREADS>), dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, lse, entropy, g_lp, g_ent, g_top, top_idx, (T*)dlogits, ldd);
+  });
 }
 
 }  // namespace
@@ -305,8 +329,8 @@ extern "C" int s2t_token_logprobs_fwd(int dtype, const void* logits, int64_t ld,
   if (rows == 0) return S2T_OK;  // (an empty tensor has no address)
   if (!logits || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index))) return S2T_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == S2T_F32) launch_fwd<float, 256>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
-  else launch_fwd<bf16_t, 256>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
+  if (dtype == S2T_F32) launch_fwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
+  else launch_fwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
   return S2T_LAUNCH_CHECK();
 }
 
@@ -319,11 +343,8 @@ extern "C" int s2t_token_logprobs_bwd(int dtype, const void* logits, int64_t ld,
   if (dtype != S2T_F32 && dtype != S2T_BF16) return S2T_ERR_DTYPE;
   if (rows == 0) return S2T_OK;
   if (!logits || !dlogits || !lse || (g_logprob && !tokens) || (g_entropy && !entropy) || (g_top && (!top_index || top == 0))) return S2T_ERR_ARG;
-  const dim3 grid((unsigned)rows);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == S2T_F32)
-    hipLaunchKernelGGL(token_logprobs_bwd_kernel<float>, grid, dim3(256), 0, s, (const float*)logits, ld, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, (float*)dlogits, ldd);
-  else
-    hipLaunchKernelGGL(token_logprobs_bwd_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t*)logits, ld, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, (bf16_t*)dlogits, ldd);
+  if (dtype == S2T_F32) launch_bwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
+  else launch_bwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
   return S2T_LAUNCH_CHECK();
 }

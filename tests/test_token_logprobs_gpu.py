@@ -50,7 +50,7 @@ def _ep(x, T):
     return E * (8 * float(z[z.isfinite()].abs().max()) + x.shape[1] / 64 + 64)
 
 
-SIZES = [(1, 1, 1), (1, 2, 2), (3, 7, 7), (5, 64, 3), (4, 257, 64), (17, 1000, 8), (60, 10000, 4), (3, 32001, 10), (2, 70001, 64), (700, 300, 1)]
+SIZES = [(1, 1, 1), (1, 2, 2), (3, 7, 7), (5, 64, 3), (4, 257, 64), (17, 1000, 8), (60, 10000, 4), (3, 32001, 10), (2, 70001, 64), (700, 300, 1), (9, 2561, 12), (5, 5121, 30), (130, 4000, 5)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -109,6 +109,9 @@ def test_gradient_against_differences():
 
 
 def test_ties_go_to_the_lowest_column_and_all_equal_rows():
+    for V in (300, 2000, 4500):  # more equal columns than are collected, for one, one and two waves to a row
+        r = Fn.token_logprobs(torch.zeros(2, V, device=DEV), top=64)
+        assert torch.equal(r.top_index[0].cpu(), torch.arange(64))
     x = torch.zeros(4, 5000, dtype=torch.bfloat16, device=DEV)
     x[1, 4000:] = 3.0
     x[2, ::7] = 1.0
@@ -123,6 +126,10 @@ def test_ties_go_to_the_lowest_column_and_all_equal_rows():
 def test_sorted_rows_in_both_directions():
     """Every candidate in one thread's reach, or spread evenly: the selection has to hold for both."""
     up = torch.arange(20000, dtype=torch.float32).mul(1e-3)
+    for n in (1000, 4000):  # (one and two waves to a row)
+        for y in (up[:n], up[:n].flip(0)):
+            r = Fn.token_logprobs(y[None].to(DEV), top=64)
+            assert torch.equal(r.top_index[0].cpu(), torch.sort(y, descending=True, stable=True).indices[:64])
     blocks = torch.zeros(20000)
     blocks[256 * torch.arange(40) + 3] = torch.arange(40, dtype=torch.float32) + 1.0      # one residue class of 256
     dense = torch.zeros(20000)
