@@ -39,7 +39,7 @@ __device__ __forceinline__ Span span_of(const s2t_paged_args& a, int b) {
 // ---- append -----------------------------------------------------------------------------------------------------------------
 // A wave takes a new token; its lanes go over the token's units: 16 bytes that pass, or two times 16 that turn together, first all of k, then
 // v, then q.  (Bound by memory, and kept busy by many small waves: two, four and eight tokens to a wave, with as many loads of each
-// lane on their way, were slower, 48, 57 and 63 us against 42 for 16 900 tokens of 4 + 4 + 16 heads x 128 in bf16, 210 MB: 5.0 TB/s.)
+// lane on their way, were slower, 48, 57 and 63 us against 42 for 17 000 tokens of 4 + 4 + 16 heads x 128 in bf16, 210 MB: 5.0 TB/s.)
 template <typename T>
 struct Turned {
   static constexpr int E = 16 / (int)sizeof(T);
@@ -114,6 +114,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 }
 
 // ---- attention --------------------------------------------------------------------------------------------------------------
+// out = softmax(scale q k^T) v in one pass over the keys, the running maximum and sum of a row carried along.
+// Single tokens are bound by the bytes of the cache (128 sequences x 8 heads of 64 over 2050 keys: 538 MB in 111 us, 4.8 TB/s; 5 tokens of
+// 16 + 4 heads of 128 over 131 000 keys: 268 MB in 51 us and 5 for the ranges), prompts by vector instructions (8 heads of 64, 8100 tokens
+// over up to 3000 keys: 59 us, 366 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
+// of five memory latencies (5.7 us).
 // A workgroup takes 16 * MT rows (new token x query head of one key/value head's group) and a range of keys, its four waves every
 // fourth tile of 32 keys; their results meet in LDS, those of several ranges in paged_combine_kernel.  Nothing but that goes through LDS:
 // the products are laid out so that what a matrix instruction returns is what the next one takes, and K and V go from the pages to
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 //                    A: lane (c, g) loads columns c * NDT .. of its 8 keys, 16 lanes a whole row, and (bf16) pairs keys by v_perm.
 // Scores, running reference and sums are fp32, in powers of two.  The reference of a row moves only when a score passes it by 2^8
 // (a vote; no exchange between lanes otherwise), so p < 2^8.  bf16 P is held as two bf16 numbers (2^-16 of the value): one rounding to
-// bf16 would add an error as large as the output's own.
+// bf16 would add an error as large as the output's own (and save 8 of 59 us with prompts, nothing where bytes count).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -164,10 +169,11 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 
 // T: type of the cache; DK: head_dim rounded up to 32, 64, 128 or 256; BIG: a half tile of 16 keys lies in one page
 // BYROWS: the four waves have 16 * MT rows each and go over all keys (n_split is 1)
+// (64 rows of 64-wide bf16 heads: held to two waves of a SIMD at the price of a spill outside the loop, 69 us instead of 96 with prompts)
 template <typename T, int DK, int MT, bool BIG, bool BYROWS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(const s2t_paged_args a, const int shift, const int group, const int spread,
-                                                              const int n_tiles, const int n_split, const float c2, const int flip,
-                                                              float* __restrict__ part) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(
+    const s2t_paged_args a, const int shift, const int group, const int spread, const int n_tiles, const int n_split, const float c2, const int flip,
+    float* __restrict__ part) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = DK / 16;          // 16-column tiles of the output
   constexpr int KE = BF ? 8 : 4;        // elements of 16 bytes
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   __shared__ float obuf[4][MT][4][64][NDT];
   __shared__ float mlbuf[4][MT][16][2];
 
-  // SPREAD: grid (8 * units, pairs / 8): all row tiles and ranges of a (sequence, key/value head) on one XCD (workgroups go round the eight),
+  // spread: grid (8 * units, pairs / 8): all row tiles and ranges of a (sequence, key/value head) on one XCD (workgroups go round the eight),
   // the longest tiles first; otherwise (pairs, units)
   const int pair = spread ? blockIdx.y * 8 + (blockIdx.x & 7) : blockIdx.x, unit = spread ? blockIdx.x >> 3 : blockIdx.y;
   if (pair >= a.B * a.kv_heads) return;
