@@ -1013,7 +1013,7 @@ def _call_on(device, name, *args):
     fn = _ENTRIES.get(name)
     if fn is None:
         fn = _ENTRIES[name] = getattr(L.lib(), name)
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):

@@ -22,7 +22,7 @@ import torch
 from . import _lib as L
 from . import kernels as K
 
-_TYPES = (torch.float32, torch.bfloat16)
+_TYPES = {torch.float32: L.S2T_F32, torch.bfloat16: L.S2T_BF16}
 _I32 = torch.int32
 
 
@@ -56,31 +56,33 @@ def _check_cache(k_pages, v_pages, page_table, lens, cu, max_new):
 
 
 def _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, q_heads):
-    """-> the fields of s2t_paged_args up to cu, head_dim, kv_heads.  One look at everything; what fails it is named by _check_cache."""
-    kind, shape, stride, of_table = k_pages.dtype, k_pages.shape, k_pages.stride(), page_table.shape
+    """-> the fields of s2t_paged_args up to cu.  One look at everything; what fails it is named by _check_cache."""
+    kind, shape, stride = k_pages.dtype, k_pages.shape, k_pages.stride()
+    of_table = page_table.shape
     if len(shape) == 4 and len(of_table) == 2:
         P, H, S, d = shape
         B, n = of_table
+        row, step = page_table.stride()
         if (kind in _TYPES and v_pages.dtype is kind and v_pages.shape == shape and v_pages.stride() == stride and stride[3] == 1
-                and P > 0 and H > 0 and S > 0 and not S & (S - 1) and not d % 16 and 16 <= d <= 256 and n > 0 and 0 < B < 65536
-                and page_table.dtype is lens.dtype is cu.dtype is _I32 and (page_table.stride(1) == 1 or n == 1)
+                and P > 0 and H > 0 and S > 0 and not S & (S - 1) and not d & 15 and 16 <= d <= 256 and n > 0 and 0 < B < 65536
+                and page_table.dtype is lens.dtype is cu.dtype is _I32 and (step == 1 or n == 1)
                 and lens.shape == (B,) and cu.shape == (B + 1,) and lens.is_contiguous() and cu.is_contiguous() and 0 <= max_new < 1 << 31
                 and N < 1 << 31):
             if q_heads < 1 or q_heads % H:
                 _refuse("%d query heads over %d key/value heads" % (q_heads, H))
-            return (L.S2T_F32 if kind is torch.float32 else L.S2T_BF16, B, N, max_new, q_heads, H, d, P, S, n, k_pages.data_ptr(),
-                    v_pages.data_ptr(), stride[0], stride[1], stride[2], page_table.data_ptr(), page_table.stride(0), lens.data_ptr(), cu.data_ptr())
+            return (_TYPES[kind], B, N, max_new, q_heads, H, d, P, S, n, k_pages.data_ptr(), v_pages.data_ptr(), stride[0], stride[1],
+                    stride[2], page_table.data_ptr(), row, lens.data_ptr(), cu.data_ptr())
     _check_cache(k_pages, v_pages, page_table, lens, cu, max_new)
     _refuse("%d rows" % N)
 
 
-def _rows(name, t, heads, like, n=None):
-    """-> address and strides of [n, heads, head_dim]."""
+def _rows(name, t, heads, kind, d, n=None):
+    """-> address and strides of [n, heads, d]."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or t.dtype is not like.dtype or shape[2] != like.shape[3] or stride[2] != 1 or (heads is not None and shape[1] != heads) \
+    if len(shape) != 3 or t.dtype is not kind or shape[2] != d or stride[2] != 1 or (heads is not None and shape[1] != heads) \
             or (n is not None and shape[0] != n):
         _refuse("%s must be [%s, %s, %d] %s with a contiguous last dimension, got %s %s" % (
-            name, "rows" if n is None else n, "heads" if heads is None else heads, like.shape[-1], like.dtype, tuple(shape), t.dtype))
+            name, "rows" if n is None else n, "heads" if heads is None else heads, d, kind, tuple(shape), t.dtype))
     return t.data_ptr(), stride[0], stride[1]
 
 
@@ -97,16 +99,19 @@ def _index(name, t, n):
     return t.data_ptr()
 
 
-def _device(k_pages, v_pages, page_table, lens, cu, x, *others):
-    """-> index of the one device that all of them (None aside) live on; ``x``: the rows that come first."""
+def _device(k_pages, v_pages, page_table, lens, cu, x, others):
+    """-> index of the one device that all of them live on; ``x``: the rows that come first."""
     dev = k_pages.get_device()
-    if not (dev == v_pages.get_device() == page_table.get_device() == lens.get_device() == cu.get_device() == x.get_device()) or dev < 0 \
-            or [1 for t in others if t is not None and t.get_device() != dev]:
-        tensors = (k_pages, v_pages, page_table, lens, cu, x) + others
+    same = dev == v_pages.get_device() == page_table.get_device() == lens.get_device() == cu.get_device() == x.get_device() and dev >= 0
+    grad = x.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+    for t in others:
+        same = same and t.get_device() == dev
+        grad = grad or t.requires_grad
+    if not same:
+        tensors = (k_pages, v_pages, page_table, lens, cu, x, *others)
         L.require_cuda(*tensors)
-        _refuse("tensors on several devices: %s" % ", ".join(str(t.device) for t in tensors if t is not None))
-    if (x.requires_grad or k_pages.requires_grad or v_pages.requires_grad or [1 for t in others if t is not None and t.requires_grad]) \
-            and torch.is_grad_enabled():
+        _refuse("tensors on several devices: %s" % ", ".join(str(t.device) for t in tensors))
+    if grad and torch.is_grad_enabled():
         raise RuntimeError("the paged cache is inference only: wrap the decoder in torch.no_grad()")
     return dev
 
@@ -120,29 +125,38 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
     into ``q_out`` (default: a new tensor; ``q`` itself: in place) and returned.
     ``rows`` (int32 [N], instead of q): new token t takes row ``rows[t]`` of k and v — the accepted drafts of a verified tree, whose
     projections the caller has kept; a row outside k is not stored."""
-    N = k.shape[0] if rows is None else rows.shape[0] if rows.dim() else -1
+    src = k.shape[0] if k.dim() else 0
+    N = src if rows is None else rows.shape[0] if rows.dim() else -1
     cache = _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, k_pages.shape[1] if q is None else q.shape[1] if q.dim() > 1 else 0)
-    kf = _rows("k", k, cache[5], k_pages)
-    vf = _rows("v", v, cache[5], k_pages, k.shape[0])
-    qf = of = _NONE3
+    kind, H, d = k_pages.dtype, cache[5], cache[6]
+    kf = _rows("k", k, H, kind, d)
+    vf = _rows("v", v, H, kind, d, src)
+    others = [v]
+    qf = of = turn = _NONE3
+    at = pick = 0
     if q is not None:
         if rows is not None:
             _refuse("q cannot be turned together with a selection of rows")
-        qf = _rows("q", q, None, k_pages, N)
-        q_out, of = _like(q) if q_out is None else (q_out, _rows("q_out", q_out, cache[4], k_pages, N))
+        qf = _rows("q", q, None, kind, d, N)
+        q_out, of = _like(q) if q_out is None else (q_out, _rows("q_out", q_out, cache[4], kind, d, N))
+        others += (q, q_out)
     elif q_out is not None:
         _refuse("q_out without q")
-    turn = _NONE3
     if rotary is not None:
         if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.shape[0] < 1 \
-                or rotary.shape[1] % 16 or not 16 <= rotary.shape[1] <= cache[6]:
+                or rotary.shape[1] % 16 or not 16 <= rotary.shape[1] <= d:
             _refuse("rotary must be float32 [positions, rot_dim], contiguous, rot_dim a multiple of 16 up to head_dim, got %s %s" % (
                 tuple(rotary.shape), rotary.dtype))
-        turn = (rotary.data_ptr(),) + tuple(rotary.shape)
-    at = _index("positions", positions, N) if positions is not None else 0
-    pick = _index("rows", rows, N) if rows is not None else 0
-    K.paged_kv_append(_device(k_pages, v_pages, page_table, lens, cu, k, v, q, rotary, positions, rows, q_out),
-                      L.PAGED_ARGS.pack(*cache, *kf, *vf, *qf, *of, *turn, at, pick, k.shape[0], *_NO_ATTENTION))
+        turn = (rotary.data_ptr(), *rotary.shape)
+        others.append(rotary)
+    if positions is not None:
+        at = _index("positions", positions, N)
+        others.append(positions)
+    if rows is not None:
+        pick = _index("rows", rows, N)
+        others.append(rows)
+    K.paged_kv_append(_device(k_pages, v_pages, page_table, lens, cu, k, others),
+                      L.PAGED_ARGS.pack(*cache, *kf, *vf, *qf, *of, *turn, at, pick, src, *_NO_ATTENTION))
     return q_out
 
 
@@ -156,29 +170,37 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
     counts its places alone, and every new token sees all of them.
     A row that sees nothing comes out 0 with lse -inf; what a row does not see never touches it, infinities and NaN included.
     Inference only.  -> out [N, q_heads, head_dim] (``out`` if given), with ``return_lse`` also the fp32 logsumexp [N, q_heads]."""
-    N, Hq, d = q.shape if q.dim() == 3 else (0, 0, 0)
+    shape = q.shape
+    N, Hq = shape[:2] if len(shape) == 3 else (0, 0)
     cache = _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, Hq)
-    qf = _rows("q", q, None, k_pages)
-    bits = _NONE3
+    kind, d = k_pages.dtype, cache[6]
+    qf = _rows("q", q, Hq, kind, d)
+    bits, others = _NONE3, ()
     if tree is not None:
         if memory:
             _refuse("a tree over a memory that holds no new tokens")
         if tree.dtype is not torch.int64 or tree.dim() != 2 or tree.shape[0] != N or tree.shape[1] < 1 or (tree.stride(1) != 1 and tree.shape[1] > 1):
             _refuse("tree must be int64 [%d, words] with contiguous rows, got %s %s" % (N, tuple(tree.shape), tree.dtype))
         bits = (tree.data_ptr(), tree.stride(0), tree.shape[1])
-    out, of = _like(q) if out is None else (out, _rows("out", out, Hq, k_pages, N))
-    dev = _device(k_pages, v_pages, page_table, lens, cu, q, tree, out)
+        others = (tree,)
+    if out is None:
+        out, of = _like(q)
+    else:
+        of = _rows("out", out, Hq, kind, d, N)
+        others += (out,)
+    dev = _device(k_pages, v_pages, page_table, lens, cu, q, others)
     lse, to_lse = None, 0
     if return_lse:
         lse = torch.empty(N, Hq, dtype=torch.float32, device=q.device)
         to_lse = lse.data_ptr()
-    tail = (to_lse, *bits, d ** -0.5 if scale is None else float(scale), 1 if memory else 0)
-    args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, 0, 0)
+    scale = d ** -0.5 if scale is None else float(scale)
+    pack = L.PAGED_ARGS.pack
+    args = pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, to_lse, *bits, scale, 1 if memory else 0, 0, 0)
     if cache[8] * cache[9] > K.PAGED_ONE_RANGE:
         n = K.paged_attention_ws_bytes(args)
         if n > 0:  # from the allocator: a captured graph keeps its own, another stream gets another
             ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-            args = L.PAGED_ARGS.pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, *tail, ws.data_ptr(), n)
+            args = pack(*cache, *_NO_KV, *qf, *_NO_APPEND, *of, to_lse, *bits, scale, 1 if memory else 0, ws.data_ptr(), n)
     K.paged_attention(dev, args)
     return (out, lse) if return_lse else out
 
