@@ -133,14 +133,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int MIN_CHUNK = 512;  // keys of a range: four tiles for each wave
 
 __device__ __forceinline__ bool finite_(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// keys of each of n_split ranges of a row tile that sees keys 0 .. kend - 1
-__device__ __forceinline__ int chunk_of(int kend, int n_split) {
-  return n_split == 1 ? max(MIN_CHUNK, kend) : max(MIN_CHUNK, ((kend + n_split - 1) / n_split + 127) & ~127);
+// keys of each of n_split ranges of a row tile that sees keys 0 .. kend - 1, at least `least` (a multiple of 128)
+__device__ __forceinline__ int chunk_of(int kend, int n_split, int least) {
+  return n_split == 1 ? max(least, kend) : max(least, ((kend + n_split - 1) / n_split + 127) & ~127);
 }
 __device__ __forceinline__ int ranges_of(int kend, int chunk) { return kend <= chunk ? 1 : (kend + chunk - 1) / chunk; }
 __device__ __forceinline__ int over(int n, int group) { return group == 1 ? n : n / group; }  // (a division is some thirty instructions)
@@ -172,7 +171,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // (64 rows of 64-wide bf16 heads: held to two waves of a SIMD at the price of a spill outside the loop, 69 us instead of 96 with prompts)
 template <typename T, int DK, int MT, bool BIG, bool BYROWS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1) void paged_attention_kernel(
-    const s2t_paged_args a, const int shift, const int group, const int spread, const int n_tiles, const int n_split, const float c2, const int flip,
+    const s2t_paged_args a, const int shift, const int group, const int spread, const int n_tiles, const int n_split, const int least, const float c2, const int flip,
     float* __restrict__ part) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = DK / 16;          // 16-column tiles of the output
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   const Span sp = span_of(a, b);
   const Reach rc = reach_of(a, sp, shift, group, row_base, 16 * MT);
   if (row_base >= rc.rows) return;
-  const int chunk = BYROWS ? 0 : chunk_of(rc.kend, n_split), used = BYROWS ? 1 : ranges_of(rc.kend, chunk);
+  const int chunk = BYROWS ? 0 : chunk_of(rc.kend, n_split, least), used = BYROWS ? 1 : ranges_of(rc.kend, chunk);
   if (split >= used) return;
   const int k_hi = BYROWS ? rc.kend : min(rc.kend, (split + 1) * chunk);
   const int all_see = rc.prefix + (a.tree ? 0 : over(row_base, group) + 1);  // every row of the tile sees the keys before this one
@@ -600,7 +599,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
 // range's columns, so that 64 * WAVES / lanes ranges are on their way at a time; the order of every sum is fixed.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args a, const int shift, const int tile_rows, const int n_split,
-                                                            const int lanes, const float* __restrict__ part) {
+                                                            const int least, const int lanes, const float* __restrict__ part) {
   __shared__ float sums[4][256];
   const int b = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6, sub = WAVES == 1 ? 0 : w;
   const int rowid = WAVES == 1 ? blockIdx.x * 4 + w : blockIdx.x;
@@ -608,7 +607,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args
   const Span sp = span_of(a, b);
   const bool live = i < min(sp.n, a.max_new);
   const Reach rc = reach_of(a, sp, shift, group, (i * group + hq % group) / tile_rows * tile_rows, tile_rows);
-  const int chunk = chunk_of(rc.kend, n_split), used = ranges_of(rc.kend, chunk);
+  const int chunk = chunk_of(rc.kend, n_split, least), used = ranges_of(rc.kend, chunk);
   if (!live || used == 1) return;  // (WAVES == 4: the whole workgroup)
   const int64_t heads = (int64_t)a.N * a.q_heads, t = sp.row0 + i, at = t * a.q_heads + hq;
   const float2* ml = reinterpret_cast<const float2*>(part + n_split * heads * d) + at;
@@ -658,7 +657,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args
 // How a call is cut: row tiles of 16 rows to a wave, whether the waves of a workgroup have rows of their own, tiles of a sequence, ranges of
 // the keys.
 struct Cut {
-  int mt, by_rows, tiles, splits;
+  int mt, by_rows, tiles, splits, least;
 };
 Cut cut_of(const s2t_paged_args* a) {
   const int64_t rows = (int64_t)a->max_new * (a->q_heads / a->kv_heads), keys = (int64_t)a->table_pages * a->page_size;
@@ -670,6 +669,7 @@ Cut cut_of(const s2t_paged_args* a) {
   c.by_rows = rows > 16 && keys <= 512 && (rows + 63) / 64 * pairs >= 256;
   if (c.by_rows) {
     c.mt = c.splits = 1;
+    c.least = 128;
     c.tiles = (int)((rows + 63) / 64);
     return c;
   }
@@ -680,8 +680,19 @@ Cut cut_of(const s2t_paged_args* a) {
   c.mt = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
   while (c.mt > 1 && (rows + 16 * c.mt - 1) / (16 * c.mt) * pairs * std::max<int64_t>(1, keys / 2048) < 256) c.mt /= 2;
   c.tiles = (int)((rows + 16 * c.mt - 1) / (16 * c.mt));
-  int64_t s = (c.mt * a->dk > 128 ? 256 : 512) / (c.tiles * pairs);
-  if (s > keys / MIN_CHUNK) s = keys / MIN_CHUNK;
+  // Ranges of the keys where there is less than a workgroup for every compute unit, as many as fill the chip and no more; each holds 128 KB
+  // of keys and values at least, as the second launch that joins them costs some 2 us.  Sequences x heads, one row each unless said:
+  //   workgroups, at most                          128     256     512   |   KB in a range       32      64     128     256    no cut
+  //   bf16, 64 wide, 4 x 16 over 4000 keys        19.2    15.0    17.0   |                     14.9    15.0    15.0    15.9    26.0 us
+  //   bf16, 64 wide, 24 x 8 over 1500             13.8    13.7    18.2   |                     13.8    13.8    13.7    13.7    13.6
+  //   bf16, 64 wide, 16 x 4 over 500               6.3     6.3     6.3   |                      7.9     8.5     6.3     6.3     6.4
+  //   bf16, 64 wide, 2 x 2 over 6000              10.3    10.4    10.4   |                      8.6     9.0    10.4    13.5    33.9
+  //   fp32, 64 wide, trees of 13, 24 x 4 over 300  9.2     9.2     9.2   |                     11.8    11.7     9.2     9.2     9.3
+  //   fp32, 128 wide, 16 x 4 over 1000            21.3    17.2    20.7   |                     17.2    17.3    17.2    19.2    26.7
+  //   fp32, 128 wide, 4 rows of 8 x 8 over 3000   40.0    30.6    38.1   |                     30.7    30.7    30.6    30.7    63.2
+  int64_t s = 256 / (c.tiles * pairs);
+  c.least = std::max(128, 131072 / (2 * a->dk * (a->dtype == S2T_F32 ? 4 : 2)) & ~127);
+  if (s > keys / c.least) s = keys / c.least;
   if (s > 256) s = 256;
   if (s < 1) s = 1;
   c.splits = (int)s;
@@ -694,8 +705,8 @@ void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
   const dim3 grid = spread ? dim3(8u * units, (unsigned)((pairs + 7) / 8)) : dim3((unsigned)pairs, (unsigned)units);
   const int shift = __builtin_ctz((unsigned)a->page_size), flip = a->scale < 0.f, group = a->q_heads / a->kv_heads;
   const float c2 = fmaxf(fabsf(a->scale) * LOG2E, 1e-30f);  // never 0: 0 times the -inf of a hidden key is not 0
-  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c2, flip, (float*)a->ws);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c2, flip, (float*)a->ws);
+  if (a->page_size >= 16) hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, true, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c.least, c2, flip, (float*)a->ws);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DK, MT, false, BYROWS>), grid, dim3(256), 0, st, *a, shift, group, spread, c.tiles, c.splits, c.least, c2, flip, (float*)a->ws);
 }
 template <typename T>
 void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
@@ -722,9 +733,9 @@ void launch_attention(const s2t_paged_args* a, const Cut& c, hipStream_t st) {
     const int rows = a->max_new * a->q_heads, shift = __builtin_ctz((unsigned)a->page_size);
     const int lanes = a->dk <= 16 ? 4 : a->dk <= 32 ? 8 : a->dk <= 64 ? 16 : a->dk <= 128 ? 32 : 64;
     if (c.splits <= 8)
-      hipLaunchKernelGGL((paged_combine_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4), (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, lanes, (const float*)a->ws);
+      hipLaunchKernelGGL((paged_combine_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4), (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, c.least, lanes, (const float*)a->ws);
     else
-      hipLaunchKernelGGL((paged_combine_kernel<T, 4>), dim3((unsigned)rows, (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, lanes, (const float*)a->ws);
+      hipLaunchKernelGGL((paged_combine_kernel<T, 4>), dim3((unsigned)rows, (unsigned)a->B), dim3(256), 0, st, *a, shift, 16 * c.mt, c.splits, c.least, lanes, (const float*)a->ws);
   }
 }
 

@@ -1022,7 +1022,7 @@ def _call_on(device, name, *args):
         L.check(status, name)
 
 
-PAGED_ONE_RANGE = 1023  # up to so many places of a sequence the attention needs no workspace (csrc/paged.hip, cut_of)
+PAGED_ONE_RANGE = 255  # up to so many places of a sequence the attention needs no workspace (csrc/paged.hip, cut_of)
 
 
 def paged_kv_append(device, args):
