@@ -519,46 +519,56 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
       for (int r = 0; r < 4; ++r) sick = fmaf(acc[mt][dt][r], 0.f, sick);
   if (__any(sick != sick)) go(std::true_type{});
 
-  // columns (4g + r) * NDT .. of query c of row tile mt: o / total, or both for paged_combine_kernel
-  auto finish = [&](int mt, int r, const float (&o)[NDT], float top, float total) {
-    const int row = row_base + mt * 16 + c, col = (4 * g + r) * NDT;
-    if (row >= rc.rows || col >= d) return;
-    const int i = tok[mt], t = sp.row0 + i, hq = h * group + row - i * group;
+  // columns col .. of a row: o / total, or both for paged_combine_kernel
+  auto finish = [&](int row, int col, const auto& o, float top, float total) {
+    constexpr int NC = sizeof(o) / 4, CH = NC < KE ? NC : KE;  // CH columns are all there or none
+    if (row >= rc.rows) return;
+    const int i = over(row, group), t = sp.row0 + i, hq = h * group + row - i * group;
     if (used == 1) {
       const float inv = total == 0.f ? 0.f : 1.f / total;  // (nothing seen; a NaN score leaves a sum of NaN, and so does its row)
       T* out = (T*)a.out + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + col;
 #pragma unroll
-      for (int dt = 0; dt < NDT; dt += 2) {
-        if constexpr (BF) *reinterpret_cast<uint32_t*>(out + dt) = bf16pack(o[dt] * inv, o[dt + 1] * inv);
-        else {
-          out[dt] = o[dt] * inv;
-          out[dt + 1] = o[dt + 1] * inv;
+      for (int e = 0; e < NC; e += CH)
+        if (col + e < d) {
+          if constexpr (BF) {
+            uint32_t y[CH / 2];
+#pragma unroll
+            for (int q = 0; q < CH / 2; ++q) y[q] = bf16pack(o[e + 2 * q] * inv, o[e + 2 * q + 1] * inv);
+            if constexpr (CH == 8) *reinterpret_cast<u32x4*>(out + e) = u32x4{y[0], y[1], y[2], y[3]};
+            else if constexpr (CH == 4) *reinterpret_cast<u32x2*>(out + e) = u32x2{y[0], y[1]};
+            else *reinterpret_cast<uint32_t*>(out + e) = y[0];
+          } else if constexpr (CH == 4) *reinterpret_cast<f32x4*>(out + e) = f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+          else *reinterpret_cast<float2*>(out + e) = make_float2(o[e] * inv, o[e + 1] * inv);
         }
-      }
       if (a.lse && col == 0) a.lse[(int64_t)t * a.q_heads + hq] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
     } else {  // part: [split][token][query head][d], then their [2]: reference and sum
       const int64_t heads = (int64_t)a.N * a.q_heads, at = split * heads + (int64_t)t * a.q_heads + hq;
       float* to = part + at * d + col;
 #pragma unroll
-      for (int dt = 0; dt < NDT; dt += 2) *reinterpret_cast<float2*>(to + dt) = make_float2(o[dt], o[dt + 1]);
+      for (int e = 0; e < NC; e += CH)
+        if (col + e < d) {
+#pragma unroll
+          for (int q = 0; q < CH; q += 2) *reinterpret_cast<float2*>(to + e + q) = make_float2(o[e + q], o[e + q + 1]);
+        }
       if (col == 0) reinterpret_cast<float2*>(part + n_split * heads * d)[at] = make_float2(top, total);
     }
   };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) l[mt] = s2t_xadd<16>(s2t_xadd<32>(l[mt]));
-  if constexpr (BYROWS) {
+  if constexpr (BYROWS) {  // the lane holds columns (4g + r) * NDT + dt of query c
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt) {
+      float o[4 * NDT];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float o[NDT];
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[dt] = acc[mt][dt][r];
-        finish(mt, r, o, m[mt], l[mt]);
-      }
+        for (int dt = 0; dt < NDT; ++dt) o[r * NDT + dt] = acc[mt][dt][r];
+      finish(row_base + mt * 16 + c, 4 * g * NDT, o, m[mt], l[mt]);
+    }
     return;
   }
-  // the four waves' results meet; wave w then finishes rows 4g + w of every 16 columns
+  // The four waves' results meet; with 64 rows each wave then finishes a row tile (its lanes write 16 columns, four of them a row), with fewer
+  // half a tile or a quarter.
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     if (g == 0) {
@@ -571,28 +581,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
       for (int dt = 0; dt < NDT; ++dt) obuf[wave][mt][r][lane][dt] = acc[mt][dt][r];
   }
   __syncthreads();
+  const int mine = wave * MT >> 2, r0 = wave * MT & 3;
+  float mw[4], top = -INFINITY;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    float mw[4], top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      mw[w] = mlbuf[w][mt][c][0];
-      top = fmaxf(top, mw[w]);
-    }
-    const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f, o[NDT];
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2_(mw[w] - ref);
-      total += f * mlbuf[w][mt][c][1];
-      if (mw[w] != -INFINITY)
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[dt] += f * obuf[w][mt][wave][lane][dt];
-    }
-    finish(mt, wave, o, top, total);
+  for (int w = 0; w < 4; ++w) {
+    mw[w] = mlbuf[w][mine][c][0];
+    top = fmaxf(top, mw[w]);
   }
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f, o[MT * NDT];
+#pragma unroll
+  for (int e = 0; e < MT * NDT; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {  // (a wave that saw nothing has sums of 0, or of NaN)
+    const float f = exp2_(mw[w] - ref);
+    total += f * mlbuf[w][mine][c][1];
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[r * NDT + dt] += f * obuf[w][mine][r0 + r][lane][dt];
+  }
+  finish(row_base + mine * 16 + c, (4 * g + r0) * NDT, o, top, total);
 }
 
 // Joins the ranges of the (new token, query head) rows, weights 2^(m - max m): WAVES waves to a row, `lanes` (a power of two) of them to a
