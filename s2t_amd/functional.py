@@ -2418,8 +2418,8 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
     V, lead = shape[-1], shape[:-1]
     if V < 1 or not 0 <= top <= min(V, 64):
         raise ValueError("token_logprobs: top = %s of a vocabulary of %d (at most 64)" % (top, V))
-    if not 0 < temperature < math.inf:
-        raise ValueError("token_logprobs: temperature must be positive, got %s" % temperature)
+    if not 1e-30 <= temperature <= 1e30:  # (its reciprocal times a logit has to be an fp32 number)
+        raise ValueError("token_logprobs: temperature must be positive (1e-30 .. 1e30), got %s" % temperature)
     if tokens is not None and (tokens.dtype is not torch.int64 or tokens.shape != lead or tokens.device != logits.device):
         raise ValueError("token_logprobs: tokens must be int64 of shape %s on %s, got %s %s on %s" % (
             tuple(lead), logits.device, tokens.dtype, tuple(tokens.shape), tokens.device))

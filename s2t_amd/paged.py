@@ -86,6 +86,19 @@ def _rows(name, t, heads, kind, d, n=None):
     return t.data_ptr(), stride[0], stride[1]
 
 
+def _no_overlap(name, t):
+    if any(n > 1 and step == 0 for n, step in zip(t.shape, t.stride())):
+        _refuse("%s to be written may not be expanded, got strides %s" % (name, t.stride()))
+
+
+def _target(name, t, heads, kind, d, n):
+    """``_rows`` of a tensor that is written."""
+    of = _rows(name, t, heads, kind, d, n)
+    if not (of[1] and of[2]):
+        _no_overlap(name, t)
+    return of
+
+
 def _like(q):
     """-> a new tensor of q's shape, its address and strides."""
     t = torch.empty_like(q)
@@ -117,7 +130,8 @@ def _device(k_pages, v_pages, page_table, lens, cu, x, others):
 
 
 def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=None, rotary=None, positions=None, rows=None, q_out=None):
-    """Stores the new tokens' keys and values ``[N, kv_heads, head_dim]`` (views of a fused projection's rows are read in place).
+    """Stores the new tokens' keys and values ``[N, kv_heads, head_dim]`` (views of a fused projection's rows are read in place; they may
+    not lie in the pages themselves, nor q_out where k or v do).
 
     ``rotary`` (float32 ``[positions, rot_dim]``: cosines, then sines; ``modules.rotary_table``) turns the first rot_dim elements of every
     key by the token's place, or by ``positions[t]`` (int32: in a tree of drafts the depth, not the place), element i together with
@@ -129,6 +143,8 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
     N = src if rows is None else rows.shape[0] if rows.dim() else -1
     cache = _cache_fields(k_pages, v_pages, page_table, lens, cu, max_new, N, k_pages.shape[1] if q is None else q.shape[1] if q.dim() > 1 else 0)
     kind, H, d = k_pages.dtype, cache[5], cache[6]
+    if not (cache[12] and cache[13] and cache[14]):
+        _no_overlap("k_pages and v_pages", k_pages)
     kf = _rows("k", k, H, kind, d)
     vf = _rows("v", v, H, kind, d, src)
     others = [v]
@@ -138,7 +154,7 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, lens, cu, max_new, q=Non
         if rows is not None:
             _refuse("q cannot be turned together with a selection of rows")
         qf = _rows("q", q, None, kind, d, N)
-        q_out, of = _like(q) if q_out is None else (q_out, _rows("q_out", q_out, cache[4], kind, d, N))
+        q_out, of = _like(q) if q_out is None else (q_out, _target("q_out", q_out, cache[4], kind, d, N))
         others += (q, q_out)
     elif q_out is not None:
         _refuse("q_out without q")
@@ -186,7 +202,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lens, cu, max_new, tree=Non
     if out is None:
         out, of = _like(q)
     else:
-        of = _rows("out", out, Hq, kind, d, N)
+        of = _target("out", out, Hq, kind, d, N)
         others += (out,)
     dev = _device(k_pages, v_pages, page_table, lens, cu, q, others)
     lse, to_lse = None, 0

@@ -560,7 +560,7 @@ class TransformerDecoderScriptable(nn.Module):
 
     def extend(self, tokens, positions, state, cu, max_new, tree=None):
         """Pushes new tokens of many sequences through the layers in one pass: ``tokens`` [N] int64, ``positions`` [N] int32 (0 for a
-        sentence's first; in a tree of drafts the depth), rows ``cu[b] .. cu[b + 1] - 1`` of sentence b, at the end of ``state.lens[b]``
+        sentence's first; in a tree of drafts the depth; below ``max_positions()``), rows ``cu[b] .. cu[b + 1] - 1`` of sentence b, at the end of ``state.lens[b]``
         places; ``tree`` as s2t_amd.paged.paged_attention takes it.  -> logits [N, V].  The new tokens' keys and values are in the cache
         afterwards, and ``state.accept`` takes over some of them in place of all."""
         if torch.is_grad_enabled():

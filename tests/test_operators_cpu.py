@@ -124,6 +124,27 @@ def test_bad_attention_calls_are_refused(change):
         _attend(**change)
 
 
+def test_expanded_targets_are_refused():
+    """One place of memory for many rows cannot be written; it can be read."""
+    for call, change in ((_attend, dict(out=torch.zeros(1, 4, 32).expand(5, 4, 32))), (_attend, dict(out=torch.zeros(5, 1, 32).expand(5, 4, 32))),
+                         (_append, dict(q=torch.zeros(5, 4, 32), q_out=torch.zeros(1, 4, 32).expand(5, 4, 32))),
+                         (_append, dict(k_pages=torch.zeros(1, 2, 16, 32).expand(7, 2, 16, 32), v_pages=torch.zeros(1, 2, 16, 32).expand(7, 2, 16, 32)))):
+        with pytest.raises(ValueError, match="expanded"):
+            call(**change)
+    one = torch.zeros(1, 2, 16, 32).expand(7, 2, 16, 32)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        _attend(k_pages=one, v_pages=one)
+    with pytest.raises(RuntimeError, match="GPU only"):  # (a dimension of one row has any stride)
+        _attend(q=torch.zeros(1, 4, 32), out=torch.zeros(4, 32).expand(1, 4, 32))
+
+
+def test_temperatures_that_fp32_cannot_divide_by_are_refused():
+    x, y = torch.zeros(4, 9), torch.zeros(4, dtype=torch.int64)
+    for t in (1e-40, 1e-320, 1e40):
+        with pytest.raises(ValueError, match="temperature"):
+            Fn.token_logprobs(x, y, temperature=t)
+
+
 def test_bad_scores_are_refused():
     x, y = torch.zeros(4, 9), torch.zeros(4, dtype=torch.int64)
     for args, kw in (((x.half(), y), {}), ((x.double(), y), {}), ((x, y.int()), {}), ((x, y[:3]), {}), ((x, y), {"top": 10}), ((x, y), {"top": -1}),
