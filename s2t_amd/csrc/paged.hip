@@ -117,8 +117,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 // out = softmax(scale q k^T) v in one pass over the keys, the running maximum and sum of a row carried along.
 // Single tokens are bound by the bytes of the cache (128 sequences x 8 heads of 64 over 2050 keys: 538 MB in 111 us, 4.8 TB/s; 5 tokens of
 // 16 + 4 heads of 128 over 131 000 keys: 268 MB in 51 us and 5 for the ranges), prompts by vector instructions (8 heads of 64, 8100 tokens
-// over up to 3000 keys: 59 us, 366 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
-// of five memory latencies (5.7 us).
+// over up to 3000 keys: 55 us, 394 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
+// of five memory latencies (5.6 us).
 // A workgroup takes 16 * MT rows (new token x query head of one key/value head's group) and a range of keys, its four waves every
 // fourth tile of 32 keys; their results meet in LDS, those of several ranges in paged_combine_kernel.  Nothing but that goes through LDS:
 // the products are laid out so that what a matrix instruction returns is what the next one takes, and K and V go from the pages to
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 //                    A: lane (c, g) loads columns c * NDT .. of its 8 keys, 16 lanes a whole row, and (bf16) pairs keys by v_perm.
 // Scores, running reference and sums are fp32, in powers of two.  The reference of a row moves only when a score passes it by 2^8
 // (a vote; no exchange between lanes otherwise), so p < 2^8.  bf16 P is held as two bf16 numbers (2^-16 of the value): one rounding to
-// bf16 would add an error as large as the output's own (and save 8 of 59 us with prompts, nothing where bytes count).
+// bf16 would add an error as large as the output's own (and save 6 of 55 us with prompts, nothing where bytes count).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
