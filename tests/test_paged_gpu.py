@@ -156,6 +156,28 @@ def test_attention_against_float64(shape, dtype, tree):
     check(c, paged.paged_attention(**on_gpu(c), tree=words.to(DEV) if tree else None, return_lse=True), sees)
 
 
+# keys in ranges (one workgroup each, joined afterwards): two ranges of 128 keys, ranges that end inside the new tokens, sequences with one range
+# next to some with several, up to 256 of them
+RANGES = [
+    ([1, 1], [255, 254], 1, 1, 256, 16),
+    ([1, 7, 2], [383, 129, 3], 2, 2, 128, 16),
+    ([40, 1, 0, 3], [230, 600, 500, 90], 2, 1, 256, 32),
+    ([3, 64], [2100, 450], 4, 1, 64, 1),
+    ([2, 1], [40000, 9], 2, 2, 16, 64),
+    ([1], [133000], 1, 1, 64, 256),
+    ([5], [33000], 4, 1, 128, 128),
+]
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", RANGES)
+def test_keys_in_ranges(shape, dtype, tree):
+    c = make(*shape, dtype=dtype, seed=500 + shape[4])
+    sees, words = random_tree(c) if tree else (None, None)
+    check(c, paged.paged_attention(**on_gpu(c), tree=words.to(DEV) if tree else None, return_lse=True), sees)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_that_see_nothing(dtype):
     """No prefix and no bits; a whole sequence of such rows next to ordinary ones; a prefix but no bits is an ordinary row."""
