@@ -844,18 +844,19 @@ int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* args);
 
 /* ------------------------------------------------------------------------------------------------
  * Scores of given tokens (sequence_scorer.py:75-110; the log_softmax + topk of search.py:113-146 per row): with z = inv_temp * logits,
- *   lse[r] = log sum exp z[r],  logprob[r] = z[r][tokens[r]] - lse[r],  entropy[r] = - sum p log p,
- *   top_index[r][0 .. top) = the columns of the largest logits, equal ones by ascending column, top_logprob their z - lse.
+ *   logprob[r] = z[r][tokens[r]] - log sum exp z[r],  entropy[r] = - sum p log p,
+ *   top_index[r][0 .. top) = the columns of the largest logits, equal ones by ascending column, top_logprob their log p;
+ *   stats[r] = (m, log2 sum 2^(c (logits - m))) with m the row's largest logit and c = inv_temp log2(e): what _bwd needs (8-byte aligned).
  * All in fp32 from one pass over the row (top <= 64).  tokens may be NULL (no logprob).  A row whose token is ignore_index scores 0,
- * top_index -1, and is not read; a token outside 0 .. V - 1 gives NaN.  Any of logprob, lse, entropy may be NULL.
- * _bwd: dlogits for upstream gradients g_logprob, g_entropy ([rows], or NULL) and g_top ([rows][top], or NULL) from the saved lse and
+ * top_index -1, and is not read; a token outside 0 .. V - 1 gives NaN.  Any of logprob, stats, entropy may be NULL.
+ * _bwd: dlogits for upstream gradients g_logprob, g_entropy ([rows], or NULL) and g_top ([rows][top], or NULL) from the saved stats and
  * entropy (needed with g_entropy only); every element of dlogits[rows][V] is written, zeros in ignored rows.
  * ------------------------------------------------------------------------------------------------ */
 int s2t_token_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore_index,
-                           float inv_temp, int top, float* logprob, float* lse, float* entropy, float* top_logprob, int64_t* top_index,
+                           float inv_temp, int top, float* logprob, float* stats, float* entropy, float* top_logprob, int64_t* top_index,
                            void* stream);
 int s2t_token_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore_index,
-                           float inv_temp, int top, const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy,
+                           float inv_temp, int top, const float* stats, const float* entropy, const float* g_logprob, const float* g_entropy,
                            const float* g_top, const int64_t* top_index, void* dlogits, int64_t ldd, void* stream);
 
 /* ---- Gradient all-reduce over RCCL / xGMI (csrc/comm.hip) ------------------------------------------------

@@ -9,15 +9,17 @@ namespace {
 constexpr int MAX_TOP = 64;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
-// Statistics of a set of z in powers of two (y = z * log2 e): maximum, s = sum 2^(y - m), t = sum 2^(y - m) (y - m).
-// lse = (m + log2 s) ln 2, entropy = (log2 s - t / s) ln 2.
+// Statistics of a set of logits in powers of two, c2 = log2(e) / T: maximum m, s = sum 2^d, t = sum 2^d d with d = c2 (x - m).
+// log p = (d - log2 s) ln 2, entropy = (log2 s - t / s) ln 2.  The difference is taken of the logits as they are: m is one of them, so that
+// rows of numbers far from zero (all of the type's lowest value, or around 10^30) lose nothing; and the backward pass is handed m and log2 s,
+// not their sum, which would hide log2 s behind a large m.
 struct Stats {
   float m, s, t;
 };
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ Stats merged(Stats a, Stats b) {
+__device__ __forceinline__ Stats merged(Stats a, Stats b, float c2) {
   const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
-  const float da = a.m - ref, db = b.m - ref, fa = exp2_(da), fb = exp2_(db);
+  const float da = (a.m - ref) * c2, db = (b.m - ref) * c2, fa = exp2_(da), fb = exp2_(db);
   // a side that fades out contributes no t either: its s * da may be infinite (maximum -inf, or the type's lowest value)
   const float ta = fa == 0.f ? 0.f : fa * (a.t + a.s * da), tb = fb == 0.f ? 0.f : fb * (b.t + b.s * db);
   return {m, a.s * fa + b.s * fb, ta + tb};
@@ -57,7 +59,7 @@ constexpr int CAND = 512;
 template <typename T, int THREADS, bool TOP, bool ENTROPY>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
                                                                  int64_t ignore, float inv_temp, int top, float* __restrict__ logprob,
-                                                                 float* __restrict__ lse_out, float* __restrict__ entropy,
+                                                                 float2* __restrict__ stats, float* __restrict__ entropy,
                                                                  float* __restrict__ top_lp, int64_t* __restrict__ top_idx) {
   constexpr int E = EPV<T>, NB = 5, WAVES = THREADS / 64;  // (five vectors of 256 threads: a row of 10 000 bf16 logits in one go)
   const int64_t r = blockIdx.x;
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
   if (tokens && y == ignore) {
     if (tid == 0) {
       if (logprob) logprob[r] = 0.f;
-      if (lse_out) lse_out[r] = 0.f;
+      if (stats) stats[r] = make_float2(0.f, 0.f);
       if (ENTROPY) entropy[r] = 0.f;
     }
     if (TOP)
@@ -88,9 +90,8 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
 #pragma unroll
     for (int e = 1; e < N; ++e) hi = fmaxf(hi, x[e]);
     if (TOP) most = fmaxf(most, hi);
-    hi *= c2;
     if (hi > st.m) {
-      const float d = st.m - hi, f = exp2_(d);
+      const float d = (st.m - hi) * c2, f = exp2_(d);
       st.t = ENTROPY && f != 0.f ? f * (st.t + st.s * d) : 0.f;
       st.s *= f;
       st.m = hi;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
     const float ref = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float d = fmaf(x[e], c2, -ref), p = exp2_(d);
+      const float d = (x[e] - ref) * c2, p = exp2_(d);
       st.s += p;
       if (ENTROPY) st.t = fmaf(p, fmaxf(d, -1e3f), st.t);  // (a column of -inf: 0 * -1e3)
     }
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
   __shared__ int winner[TOP ? THREADS : 1];
   __shared__ int n_cand, n_win;
   {  // of a wave: the common maximum, then sums
-    const float m = wave_max(st.m), ref = m == -INFINITY ? 0.f : m, d = st.m - ref, f = exp2_(d);
+    const float m = wave_max(st.m), ref = m == -INFINITY ? 0.f : m, d = (st.m - ref) * c2, f = exp2_(d);
     const float sum = wave_sum(st.s * f);
     st.t = ENTROPY ? wave_sum(f == 0.f ? 0.f : f * (st.t + st.s * d)) : 0.f;
     st.s = sum;
@@ -142,11 +143,11 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
   __syncthreads();
   st = part[0];
 #pragma unroll
-  for (int q = 1; q < WAVES; ++q) st = merged(st, part[q]);
+  for (int q = 1; q < WAVES; ++q) st = merged(st, part[q], c2);
   const float l2 = log2f(st.s);
-  auto score = [&](float x) { return (fmaf(x, c2, -st.m) - l2) * LN2; };
+  auto score = [&](float x) { return fmaf(x - st.m, inv_temp, -l2 * LN2); };  // (in nats: c2 times a difference that fp32 just holds is infinite)
   if (tid == 0) {
-    if (lse_out) lse_out[r] = (st.m + l2) * LN2;
+    if (stats) stats[r] = make_float2(st.m, l2);
     if (ENTROPY) entropy[r] = (l2 - st.t / st.s) * LN2;
     if (logprob) logprob[r] = (uint64_t)y < (uint64_t)V ? score(ld_as_f32<T>(row + y)) : __builtin_nanf("");
   }
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V,
                                                                  const int64_t* __restrict__ tokens, int64_t ignore, float inv_temp, int top,
-                                                                 const float* __restrict__ lse, const float* __restrict__ entropy,
+                                                                 const float2* __restrict__ stats, const float* __restrict__ entropy,
                                                                  const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                                                                  const float* __restrict__ g_top, const int64_t* __restrict__ top_idx,
                                                                  T* __restrict__ dlogits, int64_t ldd) {
@@ -247,10 +248,11 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const T* __
   float W = gl;
   if (g_top)
     for (int k = 0; k < top; ++k) W += g_top[r * top + k];
-  const float c2 = inv_temp * LOG2E, L2 = lse[r] * LOG2E, gw = W + ge * H, gp = ge * LN2;
+  const float c2 = inv_temp * LOG2E, gw = W + ge * H, gp = ge * LN2;
+  const float2 st = stats[r];
   // (a column of -inf: p is 0, and so is its gradient)
   auto dense = [&](float x) {
-    const float lp = fmaf(x, c2, -L2);
+    const float lp = fmaf(x - st.x, c2, -st.y);
     return -exp2_(lp) * fmaf(gp, fmaxf(lp, -1e3f), gw);
   };
   for (int v0 = tid; v0 < nvec; v0 += THREADS * NB) {
@@ -297,11 +299,11 @@ void for_threads(int64_t row_bytes, F&& f) {
 
 template <typename T>
 void launch_fwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, float* logprob,
-                float* lse, float* entropy, float* top_lp, int64_t* top_idx, hipStream_t s) {
+                float2* stats, float* entropy, float* top_lp, int64_t* top_idx, hipStream_t s) {
   for_threads((int64_t)V * sizeof(T), [&](auto n) {
     constexpr int THREADS = decltype(n)::value;
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, logprob, lse, entropy, top_lp, top_idx);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, logprob, stats, entropy, top_lp, top_idx);
     };
     if (top > 0) {
       if (entropy) go(token_logprobs_kernel<T, THREADS, true, true>);
@@ -313,41 +315,41 @@ void launch_fwd(const void* logits, int64_t ld, int64_t rows, int V, const int64
   });
 }
 template <typename T>
-void launch_bwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, const float* lse,
+void launch_bwd(const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens, int64_t ignore, float inv_temp, int top, const float2* stats,
                 const float* entropy, const float* g_lp, const float* g_ent, const float* g_top, const int64_t* top_idx, void* dlogits, int64_t ldd, hipStream_t s) {
   for_threads((int64_t)V * sizeof(T), [&](auto n) {
     constexpr int THREADS = decltype(n)::value;
-    hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, THREADS>), dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, lse, entropy, g_lp, g_ent, g_top, top_idx, (T*)dlogits, ldd);
+    hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, THREADS>), dim3((unsigned)rows), dim3(THREADS), 0, s, (const T*)logits, ld, V, tokens, ignore, inv_temp, top, stats, entropy, g_lp, g_ent, g_top, top_idx, (T*)dlogits, ldd);
   });
 }
 
 }  // namespace
 
 extern "C" int s2t_token_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens,
-                                      int64_t ignore_index, float inv_temp, int top, float* logprob, float* lse, float* entropy,
+                                      int64_t ignore_index, float inv_temp, int top, float* logprob, float* stats, float* entropy,
                                       float* top_logprob, int64_t* top_index, void* stream) {
   if (rows < 0 || rows > 0x7fffffff || V <= 0 || V > 0x7fffff00 || ld < V || top < 0 || top > V) return S2T_ERR_ARG;
   if (top > MAX_TOP) return S2T_ERR_UNSUPPORTED;
   if (dtype != S2T_F32 && dtype != S2T_BF16) return S2T_ERR_DTYPE;
   if (rows == 0) return S2T_OK;  // (an empty tensor has no address)
-  if (!logits || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index))) return S2T_ERR_ARG;
+  if (!logits || ((uintptr_t)stats & 7) || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index))) return S2T_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == S2T_F32) launch_fwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
-  else launch_fwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index, s);
+  if (dtype == S2T_F32) launch_fwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, (float2*)stats, entropy, top_logprob, top_index, s);
+  else launch_fwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, logprob, (float2*)stats, entropy, top_logprob, top_index, s);
   return S2T_LAUNCH_CHECK();
 }
 
 extern "C" int s2t_token_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int V, const int64_t* tokens,
-                                      int64_t ignore_index, float inv_temp, int top, const float* lse, const float* entropy,
+                                      int64_t ignore_index, float inv_temp, int top, const float* stats, const float* entropy,
                                       const float* g_logprob, const float* g_entropy, const float* g_top, const int64_t* top_index,
                                       void* dlogits, int64_t ldd, void* stream) {
   if (rows < 0 || rows > 0x7fffffff || V <= 0 || V > 0x7fffff00 || ld < V || ldd < V || top < 0 || top > V) return S2T_ERR_ARG;
   if (top > MAX_TOP) return S2T_ERR_UNSUPPORTED;
   if (dtype != S2T_F32 && dtype != S2T_BF16) return S2T_ERR_DTYPE;
   if (rows == 0) return S2T_OK;
-  if (!logits || !dlogits || !lse || (g_logprob && !tokens) || (g_entropy && !entropy) || (g_top && (!top_index || top == 0))) return S2T_ERR_ARG;
+  if (!logits || !dlogits || !stats || ((uintptr_t)stats & 7) || (g_logprob && !tokens) || (g_entropy && !entropy) || (g_top && (!top_index || top == 0))) return S2T_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == S2T_F32) launch_bwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
-  else launch_bwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
+  if (dtype == S2T_F32) launch_bwd<float>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, (const float2*)stats, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
+  else launch_bwd<bf16_t>(logits, ld, rows, V, tokens, ignore_index, inv_temp, top, (const float2*)stats, entropy, g_logprob, g_entropy, g_top, top_index, dlogits, ldd, s);
   return S2T_LAUNCH_CHECK();
 }

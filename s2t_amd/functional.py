@@ -2357,17 +2357,17 @@ class TokenScores(NamedTuple):
 NO_IGNORE = -(1 << 63)
 
 
-def _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, want_lse):
-    """-> logprob, entropy, top_logprob, top_index, lse of rows of logits [rows, V]; None for what is not asked for."""
+def _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, want_stats):
+    """-> logprob, entropy, top_logprob, top_index, row statistics of rows of logits [rows, V]; None for what is not asked for."""
     rows, dev = logits.shape[0], logits.device
     f32 = torch.float32
     logprob = torch.empty(rows, dtype=f32, device=dev) if tokens is not None else None
-    lse = torch.empty(rows, dtype=f32, device=dev) if want_lse else None
+    stats = torch.empty(rows, 2, dtype=f32, device=dev) if want_stats else None
     entropy = torch.empty(rows, dtype=f32, device=dev) if want_entropy else None
     top_lp = torch.empty(rows, top, dtype=f32, device=dev) if top else None
     top_idx = torch.empty(rows, top, dtype=torch.int64, device=dev) if top else None
-    K.token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_lp, top_idx)
-    return logprob, entropy, top_lp, top_idx, lse
+    K.token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, stats, entropy, top_lp, top_idx)
+    return logprob, entropy, top_lp, top_idx, stats
 
 
 class TokenLogprobsFn(torch.autograd.Function):
@@ -2376,8 +2376,8 @@ class TokenLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, ignore_index, inv_temp, top, want_entropy):
-        *out, lse = _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, True)
-        ctx.save_for_backward(logits, tokens, lse, out[1], out[3])
+        *out, stats = _score_rows(logits, tokens, ignore_index, inv_temp, top, want_entropy, True)
+        ctx.save_for_backward(logits, tokens, stats, out[1], out[3])
         ctx.args = (ignore_index, inv_temp, top)
         ctx.set_materialize_grads(False)
         if top:
@@ -2388,7 +2388,7 @@ class TokenLogprobsFn(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_top, _):
         if torch.is_grad_enabled():  # create_graph=True
             raise RuntimeError("token_logprobs is differentiable once")
-        logits, tokens, lse, entropy, top_idx = ctx.saved_tensors
+        logits, tokens, stats, entropy, top_idx = ctx.saved_tensors
         ignore_index, inv_temp, top = ctx.args
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None, None
@@ -2402,7 +2402,7 @@ class TokenLogprobsFn(torch.autograd.Function):
             g_entropy = g_entropy.contiguous()
         if g_top is not None and not g_top.is_contiguous():
             g_top = g_top.contiguous()
-        K.token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_idx, dl)
+        K.token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, stats, entropy, g_logprob, g_entropy, g_top, top_idx, dl)
         return dl, None, None, None, None, None
 
 

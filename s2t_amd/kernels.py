@@ -1038,14 +1038,14 @@ def paged_attention(device, args):
     _call_on(device, "s2t_paged_attention", args)
 
 
-def token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, lse, entropy, top_logprob, top_index):
+def token_logprobs_fwd(logits, tokens, ignore_index, inv_temp, top, logprob, stats, entropy, top_logprob, top_index):
     rows, V = logits.shape
     _call_on(logits.get_device(), "s2t_token_logprobs_fwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, _ptr(tokens),
-             ignore_index, inv_temp, top, _ptr(logprob), _ptr(lse), _ptr(entropy), _ptr(top_logprob), _ptr(top_index))
+             ignore_index, inv_temp, top, _ptr(logprob), _ptr(stats), _ptr(entropy), _ptr(top_logprob), _ptr(top_index))
 
 
-def token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, lse, entropy, g_logprob, g_entropy, g_top, top_index, dlogits):
+def token_logprobs_bwd(logits, tokens, ignore_index, inv_temp, top, stats, entropy, g_logprob, g_entropy, g_top, top_index, dlogits):
     rows, V = logits.shape
     _call_on(logits.get_device(), "s2t_token_logprobs_bwd", L.dtype_id(logits.dtype), logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V, _ptr(tokens),
-             ignore_index, inv_temp, top, _ptr(lse), _ptr(entropy), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(top_index),
+             ignore_index, inv_temp, top, _ptr(stats), _ptr(entropy), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(top_index),
              dlogits.data_ptr(), dlogits.stride(0))

@@ -290,3 +290,40 @@ def test_two_runs_are_equal_and_a_graph_replays():
         torch.cuda.synchronize()
         for a, b, c in zip(held, step(), step()):
             assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num()) and torch.equal(b, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [9, 1000, 40001])
+def test_logits_far_from_zero(V, dtype):
+    """A softmax does not change with an offset.  Rows of the type's lowest value alone, of numbers around 10^6 and -10^30, and with the type's
+    largest value have the scores and gradients of the rows' differences: within ED = e (8 max |z - max z| + V / 64 + 64) as above, a
+    difference below -200 (its p is 0 in fp32) counting as 200 where p multiplies it."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(6, V, generator=g) * 3
+    x[1] = 1e6 + x[1] * 4
+    x[2] = torch.finfo(dtype).min
+    x[3] = -1e30 + x[3]
+    x[4, V // 2] = torch.finfo(dtype).max
+    x[5] = torch.where(torch.arange(V) % 3 == 1, x[5], torch.tensor(torch.finfo(dtype).min))
+    x = x.to(dtype)
+    tokens = torch.tensor([3, 5, 7, 1, V // 2, 4])
+    ups = [torch.randn(6, generator=g), torch.randn(6, generator=g)]
+    leaf = x.to(DEV).requires_grad_()
+    r = Fn.token_logprobs(leaf, tokens.to(DEV), top=2, entropy=True)
+    (dx,) = torch.autograd.grad([r.logprob, r.entropy], leaf, [u.to(DEV) for u in ups])
+    lp, h, best, idx, grad, p, alllp = _exact(x.float(), tokens, 2, 1.0, None, ups)
+    far = (alllp - alllp.amax(1, keepdim=True)).abs().clamp(max=200)
+    ed = E * (8 * far.amax(1) + V / 64 + 64)
+    assert torch.equal(r.top_index.cpu(), idx)
+    assert bool(((r.logprob.cpu().double() - lp).abs() <= ed).all())
+    assert bool(((r.top_logprob.cpu().double() - best).abs() <= ed[:, None]).all())
+    assert bool(((r.entropy.cpu().double() - h).abs() <= ed * (2 * h + 2)).all())
+    half = E if dtype == torch.float32 else 2.0 ** -8
+    W, gh = ups[0].abs().double()[:, None], ups[1].abs().double()[:, None]
+    size = alllp.abs().clamp(max=400)
+    inner = W + gh * (size + h[:, None])
+    # a p below the smallest normal number 2^-126 may be flushed: up to 2^-126 missing, times what p is multiplied with, and the product's own
+    # flush (here p = 1.13e-38 < 2^-126 = 1.175e-38 and a factor of 43)
+    bound = half * grad.abs() + p * inner * (ed[:, None] + 16 * E) + p * gh * ed[:, None] * (2 * h[:, None] + 3) + 2.0 ** -126 * (1 + inner)
+    bound.scatter_add_(1, tokens[:, None], 4 * E * W)
+    assert bool(((dx.cpu().double() - grad).abs() <= bound).all()), ((dx.cpu().double() - grad).abs() / bound).amax(1)
