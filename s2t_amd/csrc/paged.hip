@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 // out = softmax(scale q k^T) v in one pass over the keys, the running maximum and sum of a row carried along.
 // Single tokens are bound by the bytes of the cache (128 sequences x 8 heads of 64 over 2050 keys: 538 MB in 111 us, 4.8 TB/s; 5 tokens of
 // 16 + 4 heads of 128 over 131 000 keys: 268 MB in 51 us and 5 for the ranges), prompts by vector instructions (8 heads of 64, 8100 tokens
-// over up to 3000 keys: 55 us, 394 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
+// over up to 3000 keys: 58 us, 372 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
 // of five memory latencies (5.6 us).
 // A workgroup takes 16 * MT rows (new token x query head of one key/value head's group) and a range of keys, its four waves every
 // fourth tile of 32 keys; their results meet in LDS, those of several ranges in paged_combine_kernel.  Nothing but that goes through LDS:
@@ -128,11 +128,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 //                    A: lane (c, g) loads columns c * NDT .. of its 8 keys, 16 lanes a whole row, and (bf16) pairs keys by v_perm.
 // Scores, running reference and sums are fp32, in powers of two.  The reference of a row moves only when a score passes it by 2^8
 // (a vote; no exchange between lanes otherwise), so p < 2^8.  bf16 P is held as two bf16 numbers (2^-16 of the value): one rounding to
-// bf16 would add an error as large as the output's own (and save 6 of 55 us with prompts, nothing where bytes count).
+// bf16 would add an error as large as the output's own (and save 6 of 58 us with prompts, nothing where bytes count).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOWEST = -3.402823466e38f;  // the reference of a row that has seen nothing: every score passes it, and -inf less it is -inf
 
 __device__ __forceinline__ bool finite_(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -312,11 +313,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
     constexpr bool careful = decltype(again)::value;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      m[mt] = -INFINITY;
+      m[mt] = LOWEST;
       l[mt] = 0.f;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bool huge = false;
     u32x4 kf[2][NK];
     int key0 = BYROWS ? 0 : split * chunk + 32 * wave;
     Where w;
@@ -384,34 +386,45 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
               if (!((mine >> (16 * t + r)) & 1)) s[mt][t][r] = -INFINITY;
         }
       }
-      // exponents against the references so far; one vote for all row tiles whether any of these has to move
+      // one vote for all row tiles whether a reference has to move, then the exponents.  Equal scores have equal exponents at a reference, a rounded
+      // score * c2 itself, however large it is; but where half a step of it is no longer small, the exponent of the score that it came from is not
+      // near 0 by a fused product and difference: from then on the product is rounded as the reference was.  (Exponents first, against a
+      // reference that moves by their maximum: 55 instead of 58 us with prompts, but from 2^28 on a move is lost and 2^x infinite.)
       bool grow = false;
       float top[MT];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[mt][t][r] = fmaf(s[mt][t][r], c2, -ref);
         top[mt] = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
                         fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
-        grow = grow || top[mt] > (m[mt] == -INFINITY ? -INFINITY : 8.f);
+        grow = grow || fmaf(top[mt], c2, -m[mt]) > 8.f;
       }
       if (__any(grow)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
-          const float mn = fmaxf(m[mt], ref + s2t_xmax<16>(s2t_xmax<32>(top[mt])));
-          const float move = mn == -INFINITY ? 0.f : ref - mn, fade = mn == -INFINITY ? 1.f : exp2_(m[mt] - mn);
+          const float mn = fmaxf(m[mt], s2t_xmax<16>(s2t_xmax<32>(top[mt])) * c2), fade = exp2_(m[mt] - mn);
           m[mt] = mn;
           l[mt] *= fade;
 #pragma unroll
           for (int dt = 0; dt < NDT; ++dt) acc[mt][dt] *= fade;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) s[mt][t] += move;
+          huge = huge || __any(fabsf(mn) > 0x1p20f && mn != LOWEST);
         }
       }
+      if (huge) {
+        asm volatile("");  // (a branch, not both and a choice)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[mt][t][r] *= c2;
+      }
+      const float left = huge ? 1.f : c2;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[mt][t][r] = fmaf(s[mt][t][r], left, -m[mt]);
       __builtin_amdgcn_s_setprio(1);  // (the wave that has its scores before the one that waits for keys: prompts 69.7 -> 66.7 us)
       // values: operand A of O^T
       if (exist != 0xffffffffu) {  // what lies behind the end is not to be multiplied with anything
@@ -582,19 +595,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 && MT == 4 ? 2 : 1)
   }
   __syncthreads();
   const int mine = wave * MT >> 2, r0 = wave * MT & 3;
-  float mw[4], top = -INFINITY;
+  float mw[4], top = LOWEST;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     mw[w] = mlbuf[w][mine][c][0];
     top = fmaxf(top, mw[w]);
   }
-  const float ref = top == -INFINITY ? 0.f : top;
   float total = 0.f, o[MT * NDT];
 #pragma unroll
   for (int e = 0; e < MT * NDT; ++e) o[e] = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {  // (a wave that saw nothing has sums of 0, or of NaN)
-    const float f = exp2_(mw[w] - ref);
+    const float f = exp2_(mw[w] - top);
     total += f * mlbuf[w][mine][c][1];
 #pragma unroll
     for (int r = 0; r < MT; ++r)
@@ -620,20 +632,19 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const s2t_paged_args
   if (!live || used == 1) return;  // (WAVES == 4: the whole workgroup)
   const int64_t heads = (int64_t)a.N * a.q_heads, t = sp.row0 + i, at = t * a.q_heads + hq;
   const float2* ml = reinterpret_cast<const float2*>(part + n_split * heads * d) + at;
-  float top = -INFINITY;
+  float top = LOWEST;
   for (int s = lane; s < used; s += 64) top = fmaxf(top, ml[s * heads].x);
   top = wave_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
   const int col = (lane & (lanes - 1)) * 4, first = sub * (64 / lanes) + lane / lanes, step = WAVES * (64 / lanes);
   float total = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = first; s < used; s += step) {
     const float2 x = ml[s * heads];
-    const float f = exp2_(x.x - ref);
+    const float f = exp2_(x.x - top);
     const f32x4 y = col < d ? *reinterpret_cast<const f32x4*>(part + (s * heads + at) * d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
     total += f * x.y;
-    if (x.x != -INFINITY) o += f * y;
+    o += f * y;
   }
   for (int x = lanes; x < 64; x *= 2) {
     total += __shfl_xor(total, x, 64);

@@ -266,6 +266,40 @@ def test_large_scores_and_a_scale_of_ones_own(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ctx", [20, 250, 1500, 40000])
+@pytest.mark.parametrize("power", [4, 14, 22, 31, 40, 90, 120])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_scores_of_any_size_share_the_weight(sign, power, ctx, dtype):
+    """Scores are powers of two or their double (of the other sign's: half), exact in every type: the keys of the largest score share the
+    weight to the rounding of one sum, whatever its size, and wherever among the others they stand.  out = mean of their values, within
+    A (2^-16 + 2^-21 + 2 (n + 64) e) and the rounding of the result; lse = score + log n within 2 e of its size and 2^-20."""
+    d = 64
+    c = make([3], [ctx], 2, 1, d, 16, dtype, seed=power + ctx)
+    c["q"].zero_()
+    c["q"][:, :, 5] = 2.0
+    c["k"].zero_()
+    low, high = sorted((sign * 2.0 ** power, sign * 2.0 ** (power + 1)))
+    L = ctx + 3
+    place = np.arange(L)
+    tops = torch.from_numpy(c["r"].rand(L) < 0.3)
+    tops[0] = True
+    page, slot = torch.from_numpy(c["table"][0][place // 16].astype(np.int64)), torch.from_numpy(place % 16)
+    c["k"][page, :, slot, 5] = torch.where(tops, torch.tensor(high), torch.tensor(low)).to(dtype)[:, None]
+    out, lse = paged.paged_attention(**on_gpu(c), scale=0.25, return_lse=True)
+    v = c["v"][page, 0, slot].double()
+    for i in range(3):
+        s = torch.where(tops, high / 2, low / 2)[:ctx + i + 1].double()
+        p = torch.softmax(s, 0)
+        want, A = p @ v[:ctx + i + 1], p @ v[:ctx + i + 1].abs()
+        es = 2 * E * 4 if power > 10 else 16 * E * 2.0 ** power  # (differences are either 0 or so large that the other side is 0)
+        tol = HALF[dtype] * want.abs() + A * (4 * es + 2.0 ** -16 + 2.0 ** -21 + 2 * (L + 64) * E) + 1e-37
+        l = float(torch.logsumexp(s, 0))
+        for hq in range(2):
+            assert bool(((out[i, hq].cpu().double() - want).abs() <= tol).all()), float(((out[i, hq].cpu().double() - want).abs() / tol).max())
+            assert abs(float(lse[i, hq]) - l) <= 4 * E * abs(l) + (L + 64) * E + 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_layouts_strides_and_rows_behind_the_last_sequence(dtype):
     """Pages as a view of [pages, page, heads, d], queries and outputs inside wider rows, a table inside a wider one, a loose max_new; rows
     behind the last sequence are left as they were."""
