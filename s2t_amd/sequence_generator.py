@@ -221,9 +221,13 @@ class SequenceGenerator:
                 tree = torch.tensor([_words(n.sees, words) for n in nodes], dtype=torch.int64, device=dev)
             logits = model.decoder.extend(torch.tensor([n.token for n in nodes], device=dev),
                                           i32([s.kept + n.depth for s in sents for n in s.nodes]), state, i32(cu), most, tree)
-            # five alternatives: of the best, at most pad, blank and a </s> that comes too early fall away, and <unk> may be penalised
+            # five alternatives: of the best, at most pad, blank and a </s> that comes too early fall away, and <unk> may be penalised;
+            # a bonus (a penalty below 0) may lift <unk> from any rank, so its own score comes with them
             r = _token_scores(logits, self.eos, min(5, self.vocab_size), self.temperature)
             of_eos, lps, ids = (x.tolist() for x in r)
+            if self.unk_penalty < 0:
+                of_unk = _token_scores(logits, self.unk, 0, self.temperature)[0].tolist()
+                lps, ids = [x + [y] for x, y in zip(lps, of_unk)], [x + [self.unk] for x in ids]
             at = 0
             paths = []
             for s in sents:

@@ -186,6 +186,18 @@ def test_greedy_search_with_drafts_equals_beam_one(golden_dir, kw):
                 assert g.draft_passes == 1 + (longest > 41)
 
 
+@pytest.mark.parametrize("bonus", [0.5, 2.0, 4.0, 30.0])
+def test_greedy_search_with_drafts_and_a_bonus_for_unk_equals_beam_one(golden_dir, bonus):
+    """A negative penalty lifts <unk> from any rank, below the alternatives that a pass fetches too."""
+    gen, sample, model = _golden_generator(golden_dir, unk_penalty=-bonus)
+    want = gen(beam_size=1).generate([model], sample)
+    right = [h[0]["tokens"].tolist()[:-1] for h in want]
+    assert bonus < 30 or all(t == model.decoder.dictionary.unk() for h in right for t in h)
+    for drafts in (right, [d[:1] + d[2:] for d in right], [[] for _ in right]):
+        for n in (1, 5):
+            _same_hypotheses(gen(beam_size=1, draft="ctc", draft_len=n).generate([model], sample, drafts=drafts), want)
+
+
 def test_drafts_are_refused_where_they_cannot_verify(golden_dir):
     gen, sample, model = _golden_generator(golden_dir)
     with pytest.raises(ValueError, match="beam_size 1"):
