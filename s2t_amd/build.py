@@ -1,7 +1,8 @@
 """Build libs2t_hip.so (all HIP kernels + the C-ABI) in-tree for gfx950 with hipcc.
 
 The built library lives at ``s2t_amd/lib/libs2t_hip.so`` (git-ignored, shipped to the GPU box by gpurun).
-Objects are cached by source mtime so that a rebuild after touching one kernel takes seconds.
+Objects are cached by source mtime and by the command that made them (kept beside each as ``*.cmd``), so that a rebuild after touching one
+kernel takes seconds and none of another set of flags is ever linked.
 """
 import os
 import subprocess
@@ -34,6 +35,31 @@ def _deps_mtime():
     return max(os.path.getmtime(h) for h in hs)
 
 
+def _record(cmd):
+    """``cmd`` as it is kept: the same wherever the tree lies."""
+    return "\n".join(cmd).replace(os.path.dirname(HERE), ".")
+
+
+def _current(out, cmd, inputs_mtime):
+    """Whether ``out`` is there, made by ``cmd`` and no older than what it was made of."""
+    try:
+        with open(out + ".cmd") as f:
+            return f.read() == _record(cmd) and os.path.getmtime(out) >= inputs_mtime
+    except FileNotFoundError:
+        return False
+
+
+def _make(out, cmd, failed):
+    """Runs ``cmd``, which makes ``out``; the record of the command is there only while both are whole."""
+    if os.path.exists(out + ".cmd"):
+        os.remove(out + ".cmd")
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("%s:\n%s" % (failed, r.stderr[-4000:]))
+    with open(out + ".cmd", "w") as f:
+        f.write(_record(cmd))
+
+
 def build(force=False, verbose=True):
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(LIBDIR, "obj")
@@ -44,15 +70,13 @@ def build(force=False, verbose=True):
     for src in _sources():
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), hdr):
-            jobs.append((src, obj))
+        cmd = [HIPCC] + FLAGS + FILE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        if force or not _current(obj, cmd, max(os.path.getmtime(src), hdr)):
+            jobs.append((src, obj, cmd))
 
     def cc(job):
-        src, obj = job
-        cmd = [HIPCC] + FLAGS + FILE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed for %s:\n%s" % (src, r.stderr[-4000:]))
+        src, obj, cmd = job
+        _make(obj, cmd, "hipcc failed for " + src)
         return src
 
     if jobs:
@@ -60,11 +84,9 @@ def build(force=False, verbose=True):
             for done in ex.map(cc, jobs):
                 if verbose:
                     print("[s2t_amd.build] compiled", os.path.basename(done), flush=True)
-    if jobs or not os.path.exists(LIB):
-        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed:\n" + r.stderr[-4000:])
+    cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
+    if jobs or not _current(LIB, cmd, max(os.path.getmtime(o) for o in objs)):
+        _make(LIB, cmd, "link failed")
         if verbose:
             print("[s2t_amd.build] linked", LIB, flush=True)
     return LIB
