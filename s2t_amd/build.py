@@ -25,6 +25,10 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-res
 FILE_FLAGS = {"attention_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
+def flags_of(src):
+    return FLAGS + FILE_FLAGS.get(os.path.basename(src), [])
+
+
 def _sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
@@ -70,7 +74,7 @@ def build(force=False, verbose=True):
     for src in _sources():
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        cmd = [HIPCC] + FLAGS + FILE_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
+        cmd = [HIPCC] + flags_of(src) + ["-c", src, "-o", obj]
         if force or not _current(obj, cmd, max(os.path.getmtime(src), hdr)):
             jobs.append((src, obj, cmd))
 
@@ -93,4 +97,7 @@ def build(force=False, verbose=True):
 
 
 if __name__ == "__main__":
-    build(force="--force" in sys.argv)
+    if len(sys.argv) == 3 and sys.argv[1] == "--flags":  # of one source, for a script that compiles a variant of it
+        print(" ".join(flags_of(sys.argv[2])))
+    else:
+        build(force="--force" in sys.argv)

@@ -7,7 +7,7 @@ name=$1; src=$2; shift 2
 d=s2t_amd/lib/var_$name; mkdir -p $d; objs=""
 for f in s2t_amd/csrc/*.hip; do
   o=s2t_amd/lib/obj/$(basename ${f%.hip}).o
-  if [ "$(basename $f)" = "$src" ]; then o=$d/${src%.hip}.o; /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Iinclude "$@" -c $f -o $o; fi
+  if [ "$(basename $f)" = "$src" ]; then o=$d/${src%.hip}.o; /opt/rocm/bin/hipcc $(python3 s2t_amd/build.py --flags $src) -Iinclude "$@" -c $f -o $o; fi
   objs="$objs $o"
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $d/libs2t_hip.so $objs

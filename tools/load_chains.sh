@@ -5,7 +5,7 @@
 # mask entry / statistics value where it is first used, show up as long chains.  Runs on the CPU (hipcc -S).
 src=$1; pat=${2:-.}; shift 2
 out=/tmp/chains_$$.s
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -S --cuda-device-only -I$(dirname $0)/../include "$@" s2t_amd/csrc/$src -o $out 2>/dev/null || exit 1
+/opt/rocm/bin/hipcc $(python3 s2t_amd/build.py --flags $src) -S --cuda-device-only -I$(dirname $0)/../include "$@" s2t_amd/csrc/$src -o $out 2>/dev/null || exit 1
 awk -v pat="$pat" '
   /^_Z.*:/ { if (k != "" && k ~ pat) printf "%4d round trips, %4d loads  %s\n", rt[k], nl[k], k; k=$1; pend=0 }
   /(global|buffer|scratch)_load/ && !/ lds/ { pend++; nl[k]++ }

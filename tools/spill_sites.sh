@@ -4,7 +4,7 @@
 # (the compiler's wait for the scratch load also waits for the LDS-DMA stream).  Runs on the CPU (hipcc -S).
 src=$1; pat=${2:-.}; shift 2
 out=/tmp/spill_$$.s
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -S --cuda-device-only -I$(dirname $0)/../include "$@" s2t_amd/csrc/$src -o $out 2>/dev/null || exit 1
+/opt/rocm/bin/hipcc $(python3 s2t_amd/build.py --flags $src) -S --cuda-device-only -I$(dirname $0)/../include "$@" s2t_amd/csrc/$src -o $out 2>/dev/null || exit 1
 awk -v pat="$pat" '
   /^_Z.*:/ { k=$1; inl=0 }
   /^\.LBB/ { cur=$1; inl = ($0 ~ /Loop Header|=>This/) ? 1 : 0; if (inl) loops[k SUBSEP cur]=1 }
