@@ -208,7 +208,8 @@ class SequenceGenerator:
             self.draft_passes += 1
             for b, s in enumerate(sents):
                 s.plan(self.draft_len, max_len)
-                state.cache.reserve(b, s.kept + len(s.nodes))
+                if not s.done:  # (the pages of one that is done have been given back)
+                    state.cache.reserve(b, s.kept + len(s.nodes))
             state.cache.sync()
             nodes = [n for s in sents for n in s.nodes]
             count = [len(s.nodes) for s in sents]

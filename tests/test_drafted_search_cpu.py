@@ -126,3 +126,27 @@ def test_hypotheses_are_those_of_beam_one_whatever_unk_costs(kw):
     for drafts in (right, wrong, [[] for _ in right], [r[:2] + r[3:] for r in right], right[1:] + right[:1]):
         for n in (1, 4, 30):
             _same(make(draft="ctc", draft_len=n).generate([model], _sample(4), drafts=drafts), want)
+
+
+@pytest.mark.parametrize("kw", [{}, {"draft_len": 3}])
+def test_sentences_that_are_done_hold_no_pages(kw):
+    """From the pass behind its last one on a finished sentence holds none and does not have the table copied; a pool too small for
+    all sentences at their full lengths serves them if the long ones outlive the short ones."""
+    end = [2, 4, 6, 28]
+    decoder = _Decoder(VOCAB, _random_row(end))
+    model, task = _model(decoder), _DictLike(VOCAB)
+    want = SequenceGenerator([model], task, beam_size=1, max_len_b=30).generate([model], _sample(4))
+    lengths = [len(h[0]["tokens"]) for h in want]
+    assert sorted(lengths)[-2] + 12 < max(lengths)
+    make = lambda: SequenceGenerator([model], task, beam_size=1, max_len_b=30, draft="ctc", **kw)  # noqa: E731 (of the model at hand)
+    _same(make().generate([model], _sample(4), drafts=[[]] * 4), want)   # a token to a pass
+    assert len(decoder.synced) == max(lengths)
+    for step, (dirty, held) in enumerate(decoder.synced):  # in the pass that feeds token `step` of each
+        assert [h > 0 for h in held] == [step < n for n in lengths], (step, held, lengths)
+        # a sentence gave its pages back at the end of the pass before, or one has come to a new page
+        assert dirty == (step in lengths or any(step % 4 == 0 and step < n for n in lengths)), step
+    assert any(not dirty for dirty, _ in decoder.synced[sorted(lengths)[-2] + 1:])
+    pages = -(-max(lengths) // 4) + 3                      # the longest alone, and three more
+    assert max(sum(-(-(step + 1) // 4) for n in lengths if step < n) for step in range(max(lengths))) <= pages < sum(-(-n // 4) for n in lengths)
+    model = _model(_Decoder(VOCAB, _random_row(end), pages=pages))
+    _same(make().generate([model], _sample(4), drafts=[[]] * 4), want)
