@@ -10,6 +10,7 @@ import re
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # S2T_HIP_LIB points the binding at another build of the same C-ABI (kernel experiments, a system-wide install)
@@ -194,6 +195,15 @@ def check(status: int, what: str):
     if status != 0:
         raise RuntimeError("libs2t_hip: %s failed with status %d%s" % (
             what, status, " (argument error)" if status < 0 else " (hipError_t)"))
+
+
+def refuse_tangents(what, *tensors):
+    """Raises where one of them carries a forward-mode tangent (torch.autograd.forward_ad), which a kernel called without an
+    autograd.Function would drop without a word; torch.no_grad() does not switch them off."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s: no forward-mode derivative" % what)
 
 
 def require_cuda(*tensors):

@@ -15,7 +15,7 @@ import torch
 
 from . import kernels as K
 from . import paged
-from ._lib import require_cuda
+from ._lib import refuse_tangents, require_cuda
 from .flat_params import cw, transposed
 
 _HOOKS = {"grad_ready": None}  # set by the DDP wrapper: called with a parameter once its gradient is final
@@ -2411,7 +2411,7 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
     (at most 64) best columns, equal logits in ascending order.  ``logits`` [..., V] fp32 or bf16 with any row stride (a view of
     rows padded to a multiple of 8, as the output projection returns them, is read in place), ``tokens`` [...] int64.
     Rows whose token is ``ignore_index`` score 0 (top_index -1), are not read and get no gradient; a token outside the vocabulary scores
-    NaN.  All results are fp32, differentiable with respect to the logits (once).  -> ``TokenScores``"""
+    NaN.  All results are fp32, differentiable with respect to the logits (once, in reverse mode).  -> ``TokenScores``"""
     shape = logits.shape
     if not shape or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("token_logprobs: logits [..., V] in float32 or bfloat16 expected, got %s %s" % (tuple(shape), logits.dtype))
@@ -2425,6 +2425,7 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
             tuple(lead), logits.device, tokens.dtype, tuple(tokens.shape), tokens.device))
     if tokens is None and not top and not entropy:
         raise ValueError("token_logprobs: nothing asked for (tokens, top or entropy)")
+    refuse_tangents("token_logprobs", logits)
     require_cuda(logits)
     flat = len(shape) == 2
     x = logits if flat else logits.reshape(-1, V)

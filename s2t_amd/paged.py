@@ -114,6 +114,7 @@ def _index(name, t, n):
 
 def _device(k_pages, v_pages, page_table, lens, cu, x, others):
     """-> index of the one device that all of them live on; ``x``: the rows that come first."""
+    L.refuse_tangents("paged cache", k_pages, v_pages, x, *others)
     dev = k_pages.get_device()
     same = dev == v_pages.get_device() == page_table.get_device() == lens.get_device() == cu.get_device() == x.get_device() and dev >= 0
     grad = x.requires_grad or k_pages.requires_grad or v_pages.requires_grad

@@ -155,6 +155,30 @@ def test_bad_scores_are_refused():
             Fn.token_logprobs(*args, **kw)
 
 
+def test_forward_mode_tangents_are_refused():
+    """They would be dropped without a word: by every tensor that may carry one, under no_grad too (which does not switch them off).  At a
+    dual level without tangents all is as ever."""
+    from torch.autograd import forward_ad as fa
+
+    def dual(*shape):
+        return fa.make_dual(torch.zeros(*shape), torch.ones(*shape))
+
+    y = torch.zeros(4, dtype=torch.int64)
+    with fa.dual_level():
+        calls = [lambda: Fn.token_logprobs(dual(4, 9), y), lambda: Fn.token_logprobs(dual(4, 9), entropy=True), lambda: _attend(q=dual(5, 4, 32)),
+                 lambda: _attend(k_pages=dual(7, 2, 16, 32)), lambda: _attend(v_pages=dual(7, 2, 16, 32)), lambda: _append(k=dual(5, 2, 32)),
+                 lambda: _append(v=dual(5, 2, 32)), lambda: _append(q=dual(5, 4, 32)), lambda: _append(v_pages=dual(7, 2, 16, 32)),
+                 lambda: _append(rotary=dual(8, 32))]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        for call in (_attend, _append, lambda: Fn.token_logprobs(torch.zeros(4, 9), y)):
+            with pytest.raises(RuntimeError, match="GPU only"):
+                call()
+
+
 def test_the_c_entries_refuse_before_they_launch():
     lib = L.lib()
     assert lib.s2t_paged_kv_append(None, None) == -1 and lib.s2t_paged_attention(None, None) == -1
