@@ -800,7 +800,7 @@ typedef struct s2t_paged_args {
   int32_t dtype;          /* S2T_F32 / S2T_BF16: of the pages and of q, k, v, q_out, out */
   int32_t B;              /* sequences */
   int32_t N;              /* rows of the new tokens' arrays */
-  int32_t max_new;        /* no sequence has more new tokens than this (launch bound) */
+  int32_t max_new;        /* no sequence has more new tokens than this (launch bound; at most N counts) */
   int32_t q_heads, kv_heads, dk; /* q_heads % kv_heads == 0: query head h reads key/value head h / (q_heads / kv_heads); dk % 16 == 0, <= 256 */
   int32_t num_pages, page_size, table_pages; /* table_pages: entries of a page_table row */
   void* k_pages;

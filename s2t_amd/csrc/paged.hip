@@ -768,6 +768,12 @@ int paged_args_bad(const s2t_paged_args* a) {
   if (a->dk <= 0 || a->dk % 16 || a->dk > 256) return S2T_ERR_UNSUPPORTED;
   return S2T_OK;
 }
+// A sequence brings no more new tokens than there are rows: a loose bound neither sizes a launch nor chooses how the keys are cut.
+s2t_paged_args bounded(const s2t_paged_args* a) {
+  s2t_paged_args b = *a;
+  b.max_new = std::min(b.max_new, b.N);
+  return b;
+}
 bool misaligned(const s2t_paged_args* a, const void* p, int64_t st, int64_t sh) {
   const int e = a->dtype == S2T_F32 ? 4 : 8;  // elements of 16 bytes
   return ((uintptr_t)p & 15) || st % e || sh % e;
@@ -776,8 +782,9 @@ int shift_of(const s2t_paged_args* a) { return __builtin_ctz((unsigned)a->page_s
 
 }  // namespace
 
-extern "C" int s2t_paged_kv_append(const s2t_paged_args* a, void* stream) {
-  if (int bad = paged_args_bad(a)) return bad;
+extern "C" int s2t_paged_kv_append(const s2t_paged_args* args, void* stream) {
+  if (int bad = paged_args_bad(args)) return bad;
+  const s2t_paged_args bound = bounded(args), *a = &bound;
   if ((a->q && a->rows) || (a->rows && a->src_rows < 0)) return S2T_ERR_ARG;
   if (a->rotary && (a->rot_dim <= 0 || a->rot_dim % 16 || a->rot_dim > a->dk || a->rotary_positions <= 0)) return S2T_ERR_ARG;
   if (misaligned(a, a->k_pages, a->p_sp, a->p_sh) || misaligned(a, a->v_pages, a->p_sr, 0) || misaligned(a, a->k, a->k_st, a->k_sh) ||
@@ -789,21 +796,24 @@ extern "C" int s2t_paged_kv_append(const s2t_paged_args* a, void* stream) {
   const int e = a->dtype == S2T_F32 ? 4 : 8, rot = a->rotary ? a->rot_dim : 0, units = rot / 2 / e + (a->dk - rot) / e, vecs = a->dk / e;
   if ((int64_t)std::max(a->q_heads, a->kv_heads) * vecs * vecs >= (1ll << 31)) return S2T_ERR_UNSUPPORTED;  // (divisions by reciprocals)
   const auto by = [](int n) { return n > 1 ? (uint32_t)((1ull << 32) / n + 1) : 0u; };
+  if (a->max_new > (1 << 26) - 4) return S2T_ERR_UNSUPPORTED;  // (a launch's dimension is below 2^32 threads, 64 of them to a token)
   const dim3 grid((unsigned)((a->max_new + 3) / 4), (unsigned)a->B);
   if (a->dtype == S2T_F32) hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs));
   else hipLaunchKernelGGL(paged_append_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, *a, shift_of(a), by(units), by(vecs));
   return S2T_LAUNCH_CHECK();
 }
 
-extern "C" int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* a) {
-  if (paged_args_bad(a)) return -1;
+extern "C" int64_t s2t_paged_attention_ws_bytes(const s2t_paged_args* args) {
+  if (paged_args_bad(args)) return -1;
+  const s2t_paged_args bound = bounded(args), *a = &bound;
   if (a->N == 0 || a->max_new == 0) return 0;
   const Cut c = cut_of(a);
   return c.splits > 1 ? (int64_t)c.splits * a->N * a->q_heads * (a->dk + 2) * 4 : 0;
 }
 
-extern "C" int s2t_paged_attention(const s2t_paged_args* a, void* stream) {
-  if (int bad = paged_args_bad(a)) return bad;
+extern "C" int s2t_paged_attention(const s2t_paged_args* args, void* stream) {
+  if (int bad = paged_args_bad(args)) return bad;
+  const s2t_paged_args bound = bounded(args), *a = &bound;
   if ((a->tree && (a->tree_words <= 0 || a->memory)) || !(a->scale == a->scale)) return S2T_ERR_ARG;
   if (misaligned(a, a->k_pages, a->p_sp, a->p_sh) || misaligned(a, a->v_pages, a->p_sr, 0) || misaligned(a, a->q, a->q_st, a->q_sh) ||
       misaligned(a, a->out, a->o_st, a->o_sh) || ((uintptr_t)a->tree & 7))

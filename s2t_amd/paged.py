@@ -12,7 +12,8 @@ All functions work on the tensors a serving program keeps:
 * ``page_table`` ``[seqs, n]`` int32: page of the places ``i * page_size ..`` of each sequence; unused entries may hold anything;
 * ``lens`` ``[seqs]`` int32: length of each sequence INCLUDING its new tokens;
 * ``cu`` ``[seqs + 1]`` int32: the new tokens' rows of sequence b are ``cu[b] .. cu[b + 1] - 1``, the last one at place ``lens[b] - 1``;
-* ``max_new``: no sequence brings more new tokens than this (a launch bound: later ones of a sequence are left out).
+* ``max_new``: no sequence brings more new tokens than this (a launch bound: later ones of a sequence are left out; a loose one costs empty
+  workgroups, above the number of rows it counts as that).
 
 What table, lens, cu, tree, positions and rows say is read on the device, so a captured graph serves batches of any fill; rows behind the
 last sequence are left as they were, and an entry that leads out of its bounds is never followed (include/s2t_hip.h).

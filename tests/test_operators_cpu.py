@@ -220,6 +220,32 @@ def test_the_c_entries_refuse_before_they_launch():
     assert b(0, p, 8, 1, 8, p, -1, 1.0, 2, p, None, None, None, p, None, p, 8, None) == -1  # g_top without the columns
 
 
+def test_a_bound_of_new_tokens_above_the_rows_counts_as_the_rows():
+    """It neither overflows nor changes how a call is cut (the workspace shows that); more tokens than a launch takes are refused."""
+    lib = L.lib()
+    buf = torch.zeros(64, dtype=torch.float64)
+    p = buf.data_ptr()
+    p += -p % 16
+
+    def args(N, max_new, **change):
+        a = dict(dtype=0, B=1, N=N, max_new=max_new, q_heads=2, kv_heads=1, dk=32, num_pages=1, page_size=16, table_pages=1 << 16, k_pages=p, v_pages=p,
+                 p_sp=512, p_sh=512, p_sr=32, page_table=p, table_stride=1, lens=p, cu=p, k=p, k_st=32, k_sh=32, v=p, v_st=32, v_sh=32, q=p,
+                 q_st=64, q_sh=32, q_out=p, qo_st=64, qo_sh=32, out=p, o_st=64, o_sh=32, scale=1.0)
+        a.update(change)
+        return L.PAGED_ARGS.pack(*(a.get(n) or (0.0 if n == "scale" else 0) for n in L.PAGED_FIELDS))
+
+    for N in (1, 5, 40, 700):
+        for change in ({}, dict(q_heads=8), dict(dk=128, q_st=256, q_sh=128, p_sr=128), dict(B=9)):
+            tight = lib.s2t_paged_attention_ws_bytes(args(N, N, **change))
+            assert tight > 0 or N * change.get("B", 1) > 4096   # (enough rows: no ranges)
+            for loose in (N + 1, 64 * N, 1 << 20, (1 << 31) - 1):
+                assert lib.s2t_paged_attention_ws_bytes(args(N, loose, **change)) == tight
+                assert tight == 0 or lib.s2t_paged_attention(args(N, loose, **change), None) == -1   # no workspace
+    for entry in (lib.s2t_paged_kv_append, lib.s2t_paged_attention):
+        assert entry(args(0, (1 << 31) - 1), None) == 0
+        assert entry(args((1 << 31) - 1, (1 << 31) - 1), None) == -4
+
+
 def test_pages_are_dealt_out_and_come_back():
     c = paged.PagedKVCache(2, 3, 5, 4, 1, 16, torch.float32, "cpu", page_size=8)
     c.reserve(0, 9)

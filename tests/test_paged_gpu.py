@@ -403,6 +403,29 @@ def test_append_against_float64(dtype, d, rot, page, select):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [([1, 1], [255, 900], 1, 1, 256, 16), ([2, 3, 1], [40, 9, 200], 4, 2, 64, 16), ([17, 30, 1, 0] * 16, [0, 90, 40, 7] * 16, 8, 4, 64, 16),
+                                   ([5], [33000], 4, 1, 128, 128)])
+def test_a_bound_of_new_tokens_above_the_rows_changes_nothing(shape, dtype):
+    """Bit for bit, up to the largest bound that is taken."""
+    c = make(*shape, dtype=dtype, seed=61)
+    a = on_gpu(c)
+    a["max_new"] = c["N"]
+    want = paged.paged_attention(**a, return_lse=True)
+    k, v = (torch.randn(c["N"], c["Hkv"], c["d"], generator=c["g"]).to(dtype).to(DEV) for _ in range(2))
+    pages = {}
+    for bound in (c["N"], c["N"] + 1, 1 << 24, (1 << 31) - 1):
+        a = on_gpu(c)
+        a["max_new"] = bound
+        got = paged.paged_attention(**a, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        a.pop("q")
+        paged.paged_kv_append(k, v, **a)
+        pages[bound] = (a["k_pages"], a["v_pages"])
+        assert all(torch.equal(x, y) for x, y in zip(pages[bound], pages[c["N"]]))
+    check(c, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_append_leaves_out_what_has_no_place(dtype):
     c = make([3, 2, 2], [14, 30, 4], 2, 2, 64, 16, dtype, 21)
     c["table"][1, 1] = -1                                  # sequence 1: places 16 .. do not exist
