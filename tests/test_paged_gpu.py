@@ -348,6 +348,57 @@ def test_entries_that_lead_out_of_bounds_are_never_followed(dtype):
     assert torch.isfinite(o[:3]).all()
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_length_beyond_the_table_means_all_its_keys(dtype, tree):
+    """A sequence that claims 2^30 places sees every key that its table's row holds and nothing else (its new tokens' places are not among
+    them, so a tree hides nothing), the others are bit for bit what they are without it."""
+    c = make([3, 2, 4, 3], [60, 100, 10, 0], 4, 2, 64, 16, dtype, 11)
+    c["table"][3] = np.array([3, -1, 5, 1 << 30, 0, 2, 1])[:c["table"].shape[1]]   # (pages of other sequences will do for keys)
+    assert c["table"].shape[1] == 7
+    sees, words = random_tree(c) if tree else (None, None)
+    more = dict(tree=words.to(DEV) if tree else None, return_lse=True)
+    a = on_gpu(c)
+    before = paged.paged_attention(**a, **more)
+    a["lens"][3] = 1 << 30
+    o, l = paged.paged_attention(**a, **more)
+    t = int(c["cu"][3])
+    assert torch.equal(o[:t], before[0][:t]) and torch.equal(l[:t], before[1][:t])
+    # the same keys as the prefix of a sequence whose three new tokens lie behind them and are hidden
+    c["lens"] = np.array([63, 102, 14, 112 + 3])
+    c["table"] = np.concatenate([c["table"], np.full((4, 1), -1, dtype=np.int32)], 1)
+    check(c, (o, l), sees, visible=lambda b, p: not (b == 3 and (p >= 112 or 16 <= p < 32 or 48 <= p < 64)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_that_run_backwards_or_beyond_the_rows(dtype):
+    """cu = 0, 3, 1, 900, 2 over 12 rows: sequence 0 has rows 0 - 2; sequence 1 none; sequence 2 rows 1 - 11 (11 of the 899 it claims) of
+    which ``max_new`` bounds the first four; sequence 3 none.  Row 0 has one owner and is exact; rows 5 - 11 are nobody's and stay as they
+    were; the append changes the places of the owned rows alone.  (Rows 1 - 4 come from one owner or the other.)"""
+    c = make([3, 2, 4, 3], [60, 100, 10, 0], 4, 2, 64, 16, dtype, 11)
+    a = on_gpu(c)
+    assert a["max_new"] == 4
+    a["cu"] = torch.tensor([0, 3, 1, 900, 2], dtype=torch.int32, device=DEV)
+    o = torch.full_like(a["q"], 3.0)
+    _, l = paged.paged_attention(**a, out=o, return_lse=True)
+    assert bool((o[5:] == 3).all()) and torch.isfinite(o).all()
+    out, lse, tol, ltol = exact(c)
+    assert bool(((o[0].cpu().double() - out[0]).abs() <= tol[0]).all()) and bool(((l[0].cpu().double() - lse[0]).abs() <= ltol[0]).all())
+    # sequence 2: 14 places and 11 rows, the prefix is three places, row 1 + i sees places 0 .. 3 + i; row 3 and 4 are its own alone
+    one = dict(c, B=1, N=4, news=[4], lens=np.array([7]), table=c["table"][2:3], cu=np.array([0, 4]), q=c["q"][1:5])
+    out, lse, tol, ltol = exact(one)
+    assert bool(((o[3:5].cpu().double() - out[2:]).abs() <= tol[2:]).all()) and bool(((l[3:5].cpu().double() - lse[2:]).abs() <= ltol[2:]).all())
+    k, v = (torch.randn(c["N"], 2, 64, generator=c["g"]).to(dtype) for _ in range(2))
+    want = {x: c[x].clone() for x in "kv"}
+    for b, row0, n, place in ((0, 0, 3, 60), (2, 1, 4, 3)):
+        for i in range(n):
+            for x, src in (("k", k), ("v", v)):
+                want[x][c["table"][b, (place + i) // 16], :, (place + i) % 16] = src[row0 + i]
+    a.pop("q")
+    paged.paged_kv_append(k.to(DEV), v.to(DEV), **a)
+    assert torch.equal(a["k_pages"].cpu(), want["k"]) and torch.equal(a["v_pages"].cpu(), want["v"])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("d,rot,page", [(64, 64, 16), (16, 16, 1), (48, 32, 8), (128, 128, 64), (256, 64, 2), (80, 80, 32)])
 @pytest.mark.parametrize("select", [False, True])
