@@ -594,7 +594,7 @@ class _TableCache:
     def get(self, kind, n, dim, device, dtype=torch.float32):
         key = (kind, n, dim, str(device), dtype)
         if key not in self.c:
-            t = {"sin": sinusoidal_table, "rotary": rotary_table}.get(kind, rel_pos_table)(n, dim)
+            t = sinusoidal_table(n, dim) if kind == "sin" else rel_pos_table(n, dim)
             self.c[key] = t.to(device=device, dtype=dtype)
         return self.c[key]
 
