@@ -116,9 +116,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const s2t_paged_args 
 // ---- attention --------------------------------------------------------------------------------------------------------------
 // out = softmax(scale q k^T) v in one pass over the keys, the running maximum and sum of a row carried along.
 // Single tokens are bound by the bytes of the cache (128 sequences x 8 heads of 64 over 2050 keys: 538 MB in 111 us, 4.8 TB/s; 5 tokens of
-// 16 + 4 heads of 128 over 131 000 keys: 268 MB in 51 us and 5 for the ranges), prompts by vector instructions (8 heads of 64, 8100 tokens
-// over up to 3000 keys: 58 us, 372 TFLOP/s of products; half of the vector work is exponentials and splitting p), a beam step by a chain
-// of five memory latencies (5.6 us).
+// 16 + 4 heads of 128 over 131 000 keys: 268 MB in 50 us and 5 for the ranges), prompts by vector instructions (8 heads of 64, 8100 tokens
+// over up to 3000 keys: 58 us among other work and 66 back to back, 372 and 330 TFLOP/s of products; half of the vector work is exponentials
+// and splitting p; in fp32 255 us, 85 TFLOP/s), a beam step by a chain of five memory latencies (5.6 us).  A memory of 16 sentences x 4 heads
+// of 64 under 17 rows each: 5.5 us (250 frames) and 10.6 (1000), in fp32 8.2 and 16.4, whether its heads lie side by side or apart.
 // A workgroup takes 16 * MT rows (new token x query head of one key/value head's group) and a range of keys, its four waves every
 // fourth tile of 32 keys; their results meet in LDS, those of several ranges in paged_combine_kernel.  Nothing but that goes through LDS:
 // the products are laid out so that what a matrix instruction returns is what the next one takes, and K and V go from the pages to

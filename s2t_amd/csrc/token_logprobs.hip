@@ -49,12 +49,15 @@ struct Best {
 __device__ __forceinline__ bool before(Best a, Best b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
 
 // log p_y = z_y - lse, H = -sum p log p and the best columns from one read of the row: bound by its bytes (8192 x 10000 bf16 with entropy:
-// 143 MB of rows that are not ignored in 28 us, 5.1 TB/s; 2047 x 32001 fp32 with 8 alternatives: 230 MB in 48 us, 4.8 TB/s).
+// 143 MB of rows that are not ignored in 27 us, 5.3 TB/s; 35 behind a kernel that has written 164 MB, whose lines go out as these come in,
+// 43 behind the backward pass; 2047 x 32001 fp32 with 8 alternatives: 230 MB in 48 us, 4.8 TB/s).
 // One workgroup to a row, one pass: every thread keeps the statistics of its vectors (relative to its own running maximum, moved once
 // for each NB vectors) and, for the alternatives, the maximum of its raw logits.  The top-th largest of the 64 maxima of every 64th thread
 // each bounds the alternatives from below, since as many columns reach it; the columns of the threads that reach it are read once more
-// (from the caches, dealt to all threads), those that reach it, usually hardly more than `top`, are collected and ranked by (logit, column).  Rows with more than
-// CAND such columns (ties without end) are ranked one column after the other instead.
+// (from the caches, dealt to all threads), those that reach it are collected and ranked by (logit, column).  Of independent logits 11 columns
+// reach the bound of 10 alternatives, 45 that of 32 and 90 that of 48; at 64 it is the least of the maxima, which 300 reach.  Rows with more than
+// CAND such columns (ties without end; 2 of 100 rows at 64) are ranked one column after the other instead (8192 x 10000 bf16 with 0, 10, 32,
+// 48 and 64 alternatives: 31, 41, 48, 68 and 700 us).
 constexpr int CAND = 512;
 template <typename T, int THREADS, bool TOP, bool ENTROPY>
 __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, const int64_t* __restrict__ tokens,
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const T* __rest
   }
 }
 
-// Bound by its bytes: 8192 x 10000 bf16 read (143 MB) and written (164 MB) in 49 us.
+// Bound by its bytes: 8192 x 10000 bf16 read (143 MB) and written (164 MB) in 50 us.
 // d logits of one row: -p (W + g_entropy (log p + H)) / T with W = g_logprob + sum g_top; the thread that stored the column of the token or of
 // an alternative stores it once more with its own gradient added before the rounding.
 template <typename T, int THREADS>
